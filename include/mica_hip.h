@@ -14,7 +14,8 @@
  *     data_ptr()); h_* is HOST memory.  `stream` is a hipStream_t passed as void* (NULL = default).
  *   - one mica_ctx per GPU; a ctx is not thread-safe, different ctxs are independent.
  *   - kernels are launched on `stream`.  Which calls return before the device work is done is stated per function:
- *       asynchronous (enqueue and return): mica_gather_tiles(_u8), mica_stitch_tiles, mica_postprocess;
+ *       asynchronous (enqueue and return): mica_gather_tiles(_u8), mica_stitch_tiles, mica_postprocess, mica_token_logprobs(_backward),
+ *       mica_distill_loss / _backward / _step (these five can be captured into a graph);
  *       SYNCHRONISE `stream` before returning: mica_forward_logits / _tiles / _records (they read back the per-tile |AF3| sums that
  *       pick the branch of models/model.py:56-63 and the per-tile range flags of the split-f16 encoding, and may repeat a tile, see
  *       mica_get_last_forward_scale), mica_finalize_weights, mica_normalise_map*, mica_zoom_cubic*, mica_rasterise_atoms, the point-list
@@ -51,7 +52,7 @@ typedef struct mica_ctx mica_ctx;
 #define MICA_AF_ALWAYS 3    /* no test: every tile takes the AF3 branch - for a caller that cut one batch into several calls and
                                evaluated the batch-wide test itself (mica_amd/engine.py does for batches beyond max_batch)      */
 
-int mica_abi_version(void);   /* 3 (round 6: mica_get_last_forward_input_runs, mica_get_last_forward_af_tiles); bumped with every export or struct change */
+int mica_abi_version(void);   /* 4 (3: mica_get_last_forward_input_runs, mica_get_last_forward_af_tiles; 4: mica_token_logprobs*, mica_distill_*); bumped with every export or struct change */
 
 /* ---- context ---------------------------------------------------------------------------- */
 /* Allocates the activation workspace for up to max_batch tiles of tile_size^3 voxels in flight (about 4.6 GB per 64^3 tile).
@@ -235,6 +236,67 @@ int mica_neighbour_matrix(mica_ctx* ctx, const double* d_cands, int64_t n, const
 #endif
 int mica_neighbour_matrix_np(mica_ctx* ctx, const double* d_cands, int64_t n, const float* d_bb, int64_t n0, int64_t n1, int64_t n2,
                              int numpy_rules, double* d_dis, double* d_mat, void* stream);
+
+/* ---- scoring of class distributions, and distillation from a teacher's top alternatives ------- */
+/* Rows of logits in any of three types, read where they are.  Row (o, i) begins at element o * stride_outer + i * stride_inner, its
+ * class v lies stride_class * v further on.  class_last says how the results with a class or list axis are laid out: 1 = C-contiguous
+ * [outer][inner][classes or K], 0 = [outer][classes or K][inner] (NCDHW logits of a head: outer = batch, inner = voxels).
+ * More than 64 classes: class_last = 1 and stride_class = 1 only.  Limits: 1 <= classes <= 2^28, outer * inner < 2^31.          */
+#define MICA_F32 0
+#define MICA_BF16 1
+#define MICA_F16 2
+typedef struct mica_logits {
+    const void* d_data;
+    int32_t dtype;              /* MICA_F32 / MICA_BF16 / MICA_F16 */
+    int32_t class_last;
+    int64_t outer, inner, classes;
+    int64_t stride_outer, stride_inner, stride_class;      /* in elements, >= 0 */
+} mica_logits;
+/* Per row, y = z / temperature (temperature in [1e-4, 1e4]), everything in float32:
+ *   d_lse      log sum_v e^{y_v}
+ *   d_logprob  y_t - lse of the given token t (d_tokens: token_bytes 4 or 8; both nullable together); t == ignore_index: 0;
+ *              t outside [0, classes): NaN
+ *   d_entropy  -sum_v p_v log p_v
+ *   d_top_index int32 / d_top_logprob: the `top` (0 .. min(64, classes)) largest logits, ties to the lowest class, -0 = +0, NaN below
+ *              every number; nullable together when top = 0
+ * A row without a finite class (every logit -inf): lse and log probabilities -inf, entropy 0, alternatives 0, 1, 2 ...  A NaN or +inf
+ * among a row's logits makes its results NaN (the alternatives' indices stay valid and distinct).  d_ws: workspace of
+ * mica_token_logprobs_ws() bytes, 16-byte aligned, free again when the stream has passed the call (nullable if 0 bytes).             */
+int64_t mica_token_logprobs_ws(const mica_logits* z, int top);      /* bytes; < 0: the view is refused */
+int mica_token_logprobs(mica_ctx* ctx, const mica_logits* z, const void* d_tokens, int token_bytes, int64_t ignore_index, float temperature,
+                        int top, float* d_logprob, float* d_entropy, float* d_lse, float* d_top_logprob, int32_t* d_top_index,
+                        void* d_ws, int64_t ws_bytes, void* stream);
+/* d_grad (the logits' type, laid out as class_last says) = gradient of sum_n g_logprob logprob + g_entropy entropy + g_lse lse; each of
+ * the three upstream gradients f32[rows] is nullable.  d_lse, d_entropy: what the forward call wrote.  0 in a row without a finite
+ * class; a token out of range makes its row's gradient NaN.                                                                       */
+int mica_token_logprobs_backward(mica_ctx* ctx, const mica_logits* z, const void* d_tokens, int token_bytes, int64_t ignore_index,
+                                 float temperature, const float* d_lse, const float* d_entropy, const float* d_g_logprob,
+                                 const float* d_g_entropy, const float* d_g_lse, void* d_grad, void* stream);
+/* A teacher's K (1 .. 256) alternatives per row, C-contiguous [outer][inner][K] or [outer][K][inner] as the logits' class_last says:
+ * d_index (4- or 8-byte integers, negative = unused entry), d_value = their log probabilities at the loss's temperature.  A class named
+ * twice counts with both its entries.  tail = 0: p = the values' softmax over the K entries (any constant per row cancels).  tail = 1:
+ * p_k = e^{value_k}, and the classes that are not listed share the rest r = max(0, 1 - sum p) as one alternative.                   */
+typedef struct mica_top_list {
+    const void* d_index;
+    const void* d_value;
+    int32_t index_bytes;
+    int32_t value_dtype;
+    int32_t k;
+    int32_t tail;
+} mica_top_list;
+/* d_loss f32[rows] = T^2 [ sum_k p_k (log p_k - log q_{index_k}) + r (log r - log q_rest) ], q = softmax(z / T).  0 for a row whose
+ * entries are all unused; +inf (with gradient 0) where the student's row has no finite class; NaN for an index >= classes.
+ * d_aux f32[4][rows] (nullable) is what mica_distill_backward reads; not written, and not read there, for classes <= 64.          */
+int64_t mica_distill_ws(const mica_logits* z, int step);            /* bytes for mica_distill_loss (step = 0) / mica_distill_step (1) */
+int mica_distill_loss(mica_ctx* ctx, const mica_logits* z, const mica_top_list* list, float temperature, float* d_loss, float* d_aux,
+                      void* d_ws, int64_t ws_bytes, void* stream);
+/* d_grad = gradient of sum_n g_loss loss with respect to the logits */
+int mica_distill_backward(mica_ctx* ctx, const mica_logits* z, const mica_top_list* list, float temperature, const float* d_aux,
+                          const float* d_g_loss, void* d_grad, void* stream);
+/* Loss and gradient of a training step in one call: d_loss = weight loss, d_grad = gradient of sum_n weight_n loss_n; d_weight f32[rows]
+ * nullable (1); a row of weight 0 has loss and gradient 0 whatever it holds.                                                       */
+int mica_distill_step(mica_ctx* ctx, const mica_logits* z, const mica_top_list* list, float temperature, const float* d_weight,
+                      float* d_loss, void* d_grad, void* d_ws, int64_t ws_bytes, void* stream);
 
 /* ---- single-op entry points (parity tests drive each kernel through the ABI) -------------- */
 /* Box limits of all of them: 1 <= batch <= 64 and every edge d, h, w in [1, 128] (the edges mica_create_dims admits: the conv

@@ -8,16 +8,31 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libmica_hip.so")
 
-ABI_VERSION = 3          # mica_abi_version() of the library these signatures describe (bumped whenever an export or a struct changes)
+ABI_VERSION = 4          # mica_abi_version() of the library these signatures describe (bumped whenever an export or a struct changes)
 MICA_OK = 0
 MICA_ERR_ARG, MICA_ERR_HIP, MICA_ERR_STATE, MICA_ERR_RANGE = -1, -2, -3, -4
 AF_NONE, AF_PER_TILE, AF_BATCH, AF_ALWAYS = 0, 1, 2, 3
+
+MICA_F32, MICA_BF16, MICA_F16 = 0, 1, 2      # types of the scoring entry points
+
+
+class MicaLogits(C.Structure):
+    _fields_ = [("d_data", C.c_void_p), ("dtype", C.c_int32), ("class_last", C.c_int32), ("outer", C.c_int64), ("inner", C.c_int64),
+                ("classes", C.c_int64), ("stride_outer", C.c_int64), ("stride_inner", C.c_int64), ("stride_class", C.c_int64)]
+
+
+class MicaTopList(C.Structure):
+    _fields_ = [("d_index", C.c_void_p), ("d_value", C.c_void_p), ("index_bytes", C.c_int32), ("value_dtype", C.c_int32), ("k", C.c_int32),
+                ("tail", C.c_int32)]
+
 
 _P = C.c_void_p
 _I, _L, _F = C.c_int, C.c_int64, C.c_float
 _FP = C.POINTER(C.c_float)
 _LP = C.POINTER(C.c_int64)
 _DP = C.POINTER(C.c_double)
+_ZP = C.POINTER(MicaLogits)
+_TP = C.POINTER(MicaTopList)
 
 # name -> (restype, argtypes): every symbol include/mica_hip.h declares
 SIGNATURES = {
@@ -52,6 +67,13 @@ SIGNATURES = {
     "mica_nms_points": (_I, [_P, _P, _L, _L, _L, _L, C.c_double, _P, _P]),
     "mica_neighbour_matrix": (_I, [_P, _P, _L, _P, _L, _L, _L, _P, _P, _P]),
     "mica_neighbour_matrix_np": (_I, [_P, _P, _L, _P, _L, _L, _L, _I, _P, _P, _P]),
+    "mica_token_logprobs_ws": (_L, [_ZP, _I]),
+    "mica_token_logprobs": (_I, [_P, _ZP, _P, _I, _L, _F, _I, _P, _P, _P, _P, _P, _P, _L, _P]),
+    "mica_token_logprobs_backward": (_I, [_P, _ZP, _P, _I, _L, _F, _P, _P, _P, _P, _P, _P, _P]),
+    "mica_distill_ws": (_L, [_ZP, _I]),
+    "mica_distill_loss": (_I, [_P, _ZP, _TP, _F, _P, _P, _P, _L, _P]),
+    "mica_distill_backward": (_I, [_P, _ZP, _TP, _F, _P, _P, _P, _P]),
+    "mica_distill_step": (_I, [_P, _ZP, _TP, _F, _P, _P, _P, _P, _L, _P]),
     "mica_op_conv3d": (_I, [_P, _P, _I, _I, _I, _I, _I, _FP, _FP, _I, _I, _P, _P]),
     "mica_op_norm_conv1_conv3": (_I, [_P, _P, _I, _I, _I, _I, _I, _FP, _FP, _I, _FP, _FP, _I, _P, _P]),
     "mica_op_conv3d_variant": (_I, [_P, _P, _I, _I, _I, _I, _I, _FP, _FP, _I, _I, _I, _P, _P]),

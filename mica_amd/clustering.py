@@ -11,6 +11,7 @@ with the caller, and so do the scalar decisions on per-cluster numbers and the s
     CA_cands = nms(eng, ca, pts, val_mat, vol_shape, thr, r)     # :799-831
     new_cands, new_AAs, kept = refine(eng, vols, CA_cands)       # :834-858
     dis, lists, neigh_mat = neighbours(eng, vols, new_cands)     # :860-888
+    fit = residue_scores(eng, new_AAs, residues, top=3)          # log probabilities of assigned residues, entropy, alternatives
 """
 from __future__ import annotations
 
@@ -41,6 +42,15 @@ def refine(engine, volumes: dict, ca_cands):
     coord, aao, ok = engine.refine_candidates(ca, aa.contiguous(), c)
     ok = ok.cpu().numpy()
     return coord.cpu().numpy()[ok], aao.cpu().numpy()[ok], np.nonzero(ok)[0]
+
+
+def residue_scores(engine, new_AAs, residues=None, top: int = 3):
+    """How well residues fit the refined candidates: new_AAs float [m, 20] profiles as `refine` returns them (any positive scale per
+    row; host array or device tensor) -> scoring.TokenScores of the normalised profiles on the device: log probability of `residues`
+    (integers [m], -100 = none; e.g. the sequence a trace assigns), entropy, and the `top` residues in order."""
+    aa = torch.as_tensor(new_AAs).to(engine.device, torch.float32)
+    tok = None if residues is None else torch.as_tensor(residues).to(engine.device, torch.int64)
+    return engine.token_logprobs(torch.log(aa), tok, top=top)
 
 
 def gather_at(engine, vol: torch.Tensor, pts):

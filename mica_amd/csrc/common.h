@@ -275,6 +275,26 @@ int refine_candidates_device(const float* d_ca, const float* d_aa, int n0, int n
 // modeler.py:776-787 (np.sum per cluster, numpy's summation order), :822-831 (greedy NMS over sorted candidates), :860-888
 int segment_sums_device(const float* d_vals, const int64_t* d_seg_off, int64_t nseg, float* d_sums, hipStream_t st, char* err, int errlen);
 int nms_points_device(const int* d_pts, int64_t n, int n0, int n1, int n2, double radius, int* d_keep, hipStream_t st, char* err, int errlen);
+// class scoring and distillation (kernels_score.hip); the entry points have checked the view
+constexpr int SCORE_COL_MAX = 64;            // up to here a thread holds all classes of a row in registers
+constexpr int SCORE_SEG_MAX = 131072;        // classes one block streams (a bit per class in LDS: 16 KB)
+struct LogitsView { const void* p; int dtype, class_last; int64_t outer, inner, classes, so, si, sc; };
+struct DistillList { const void* index; const void* teacher; int index_bytes, teacher_dtype, k, tail; };
+struct SegPlan { int n, len; };              // a row is cut into n segments of len classes
+bool score_is_col(const LogitsView& v);
+SegPlan score_segments(const LogitsView& v, int64_t rows);
+int64_t score_ws_bytes(const LogitsView& v, int64_t rows, int top);
+int64_t distill_ws_bytes(const LogitsView& v, int64_t rows, bool step);
+void launch_score(const LogitsView& v, int64_t rows, const void* tokens, int token_bytes, int64_t ignore, float temperature, int top, float* logprob,
+                  float* entropy, float* lse, float* top_logprob, int* top_index, void* ws, hipStream_t st);
+void launch_score_grad(const LogitsView& v, int64_t rows, const void* tokens, int token_bytes, int64_t ignore, float temperature, const float* lse,
+                       const float* entropy, const float* g_logprob, const float* g_entropy, const float* g_lse, void* grad, hipStream_t st);
+void launch_distill_loss(const LogitsView& v, int64_t rows, const DistillList& d, float temperature, float* loss, float* aux, void* ws, hipStream_t st);
+void launch_distill_grad(const LogitsView& v, int64_t rows, const DistillList& d, float temperature, const float* aux, const float* g_loss, void* grad,
+                         hipStream_t st);
+void launch_distill_step(const LogitsView& v, int64_t rows, const DistillList& d, float temperature, const float* weight, float* loss, void* grad, void* ws,
+                         hipStream_t st);
+
 int neighbour_matrix_device(const double* d_cands, int64_t n, const float* d_bb, int n0, int n1, int n2, double* d_dis, double* d_mat,
                             int legacy, hipStream_t st, char* err, int errlen);
 

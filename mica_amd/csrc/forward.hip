@@ -631,7 +631,7 @@ static int forward_checked(mica_ctx* c, const float* d_map, const float* d_af, i
 // =================================================================================================
 extern "C" {
 
-int mica_abi_version(void) { return 3; }
+int mica_abi_version(void) { return 4; }
 
 const char* mica_last_error(const mica_ctx* ctx) { return ctx ? ctx->err.c_str() : g_create_err.c_str(); }
 
@@ -1413,6 +1413,160 @@ int mica_get_profile(mica_ctx* c, int kind, double* h_ms_total, int64_t* h_launc
 
 int mica_get_conv_profile(mica_ctx* c, double* h_ms_total, int64_t* h_launches, double* h_flops) {
     return mica_get_profile(c, 0, h_ms_total, h_launches, h_flops);
+}
+
+// ---- class scoring and distillation (kernels_score.hip) ----
+namespace {
+// the calling thread's current device is put back when the call returns
+struct DeviceGuard {
+    int prev = -1;
+    DeviceGuard() { if (hipGetDevice(&prev) != hipSuccess) prev = -1; }
+    ~DeviceGuard() { int now = -1; if (prev >= 0 && hipGetDevice(&now) == hipSuccess && now != prev) (void)hipSetDevice(prev); }
+};
+// nullptr, or why a view is refused; an empty view (no rows) is fine
+const char* logits_view(const mica_logits* z, LogitsView& v, int64_t& rows) {
+    if (!z) return "null logits";
+    if (z->dtype != MICA_F32 && z->dtype != MICA_BF16 && z->dtype != MICA_F16) return "unknown logits dtype";
+    if (z->classes < 1 || z->classes > ((int64_t)1 << 28)) return "classes must be in [1, 2^28]";
+    if (z->outer < 0 || z->inner < 0 || z->outer > 0x7FFFFFFF || z->inner > 0x7FFFFFFF || z->outer * z->inner > 0x7FFFFFFF) return "outer * inner must be below 2^31";
+    if (z->stride_outer < 0 || z->stride_inner < 0 || z->stride_class < 0) return "negative stride";
+    if (z->classes > SCORE_COL_MAX && (z->stride_class != 1 || !z->class_last)) return "more than 64 classes have to be contiguous and last";
+    rows = z->outer * z->inner;
+    if (rows > 0 && (!z->d_data || ((uintptr_t)z->d_data % (z->dtype == MICA_F32 ? 4 : 2)))) return "null or misaligned logits";
+    if (z->classes > SCORE_COL_MAX && rows * ((z->classes + SCORE_COL_MAX - 1) / 4096 + 1) > 0x7FFFFFFF) return "too many rows of this length";
+    v = LogitsView{z->d_data, z->dtype, z->class_last ? 1 : 0, z->outer, z->inner, z->classes, z->stride_outer, z->stride_inner, z->stride_class};
+    return nullptr;
+}
+const char* top_list(const mica_top_list* t, int64_t rows, DistillList& d) {
+    if (!t) return "null teacher list";
+    if (t->k < 1 || t->k > 256) return "the teacher's list must have 1 to 256 entries";
+    if (t->index_bytes != 4 && t->index_bytes != 8) return "index_bytes must be 4 or 8";
+    if (t->value_dtype != MICA_F32 && t->value_dtype != MICA_BF16 && t->value_dtype != MICA_F16) return "unknown teacher dtype";
+    if (rows > 0 && (!t->d_index || !t->d_value)) return "null teacher list";
+    d = DistillList{t->d_index, t->d_value, t->index_bytes, t->value_dtype, t->k, t->tail ? 1 : 0};
+    return nullptr;
+}
+bool bad_temperature(float t) { return !(t >= 1e-4f && t <= 1e4f); }
+}  // namespace
+
+#define SCORE_REFUSE(c, name, why)                                  \
+    do {                                                            \
+        (c)->err = std::string(name ": ") + (why);                  \
+        return MICA_ERR_ARG;                                        \
+    } while (0)
+
+int64_t mica_token_logprobs_ws(const mica_logits* z, int top) {
+    LogitsView v;
+    int64_t rows = 0;
+    if (logits_view(z, v, rows) || top < 0 || top > 64 || top > v.classes) return MICA_ERR_ARG;
+    return rows ? score_ws_bytes(v, rows, top) : 0;
+}
+
+int mica_token_logprobs(mica_ctx* c, const mica_logits* z, const void* d_tokens, int token_bytes, int64_t ignore_index, float temperature, int top,
+                        float* d_logprob, float* d_entropy, float* d_lse, float* d_top_logprob, int32_t* d_top_index, void* d_ws, int64_t ws_bytes,
+                        void* stream) {
+    if (!c) return MICA_ERR_ARG;
+    LogitsView v;
+    int64_t rows = 0;
+    if (const char* why = logits_view(z, v, rows)) SCORE_REFUSE(c, "mica_token_logprobs", why);
+    if (bad_temperature(temperature)) SCORE_REFUSE(c, "mica_token_logprobs", "temperature must be in [1e-4, 1e4]");
+    if (top < 0 || top > 64 || top > v.classes) SCORE_REFUSE(c, "mica_token_logprobs", "top must be in [0, min(64, classes)]");
+    if (!rows) return MICA_OK;
+    if (!d_entropy || !d_lse || (d_tokens == nullptr) != (d_logprob == nullptr) || (d_tokens && token_bytes != 4 && token_bytes != 8) ||
+        (top > 0 && (!d_top_logprob || !d_top_index)))
+        SCORE_REFUSE(c, "mica_token_logprobs", "null pointer or token size");
+    const int64_t need = score_ws_bytes(v, rows, top);
+    if (need > 0 && (!d_ws || ws_bytes < need || ((uintptr_t)d_ws & 15))) SCORE_REFUSE(c, "mica_token_logprobs", "workspace too small or misaligned");
+    DeviceGuard guard;
+    MICA_ENTER(c);
+    launch_score(v, rows, d_tokens, token_bytes, ignore_index, temperature, top, d_logprob, d_entropy, d_lse, d_top_logprob, d_top_index, d_ws,
+                 (hipStream_t)stream);
+    CHECK_LAUNCHES(c);
+    return MICA_OK;
+}
+
+int mica_token_logprobs_backward(mica_ctx* c, const mica_logits* z, const void* d_tokens, int token_bytes, int64_t ignore_index, float temperature,
+                                 const float* d_lse, const float* d_entropy, const float* d_g_logprob, const float* d_g_entropy, const float* d_g_lse,
+                                 void* d_grad, void* stream) {
+    if (!c) return MICA_ERR_ARG;
+    LogitsView v;
+    int64_t rows = 0;
+    if (const char* why = logits_view(z, v, rows)) SCORE_REFUSE(c, "mica_token_logprobs_backward", why);
+    if (bad_temperature(temperature)) SCORE_REFUSE(c, "mica_token_logprobs_backward", "temperature must be in [1e-4, 1e4]");
+    if (!rows) return MICA_OK;
+    if (!d_lse || !d_entropy || !d_grad || (d_g_logprob && (!d_tokens || (token_bytes != 4 && token_bytes != 8))))
+        SCORE_REFUSE(c, "mica_token_logprobs_backward", "null pointer or token size");
+    DeviceGuard guard;
+    MICA_ENTER(c);
+    launch_score_grad(v, rows, d_tokens, token_bytes, ignore_index, temperature, d_lse, d_entropy, d_g_logprob, d_g_entropy, d_g_lse, d_grad,
+                      (hipStream_t)stream);
+    CHECK_LAUNCHES(c);
+    return MICA_OK;
+}
+
+int64_t mica_distill_ws(const mica_logits* z, int step) {
+    LogitsView v;
+    int64_t rows = 0;
+    if (logits_view(z, v, rows)) return MICA_ERR_ARG;
+    return rows ? distill_ws_bytes(v, rows, step != 0) : 0;
+}
+
+int mica_distill_loss(mica_ctx* c, const mica_logits* z, const mica_top_list* list, float temperature, float* d_loss, float* d_aux, void* d_ws,
+                      int64_t ws_bytes, void* stream) {
+    if (!c) return MICA_ERR_ARG;
+    LogitsView v;
+    DistillList d;
+    int64_t rows = 0;
+    if (const char* why = logits_view(z, v, rows)) SCORE_REFUSE(c, "mica_distill_loss", why);
+    if (const char* why = top_list(list, rows, d)) SCORE_REFUSE(c, "mica_distill_loss", why);
+    if (bad_temperature(temperature)) SCORE_REFUSE(c, "mica_distill_loss", "temperature must be in [1e-4, 1e4]");
+    if (!rows) return MICA_OK;
+    if (!d_loss) SCORE_REFUSE(c, "mica_distill_loss", "null pointer");
+    const int64_t need = distill_ws_bytes(v, rows, false);
+    if (need > 0 && (!d_ws || ws_bytes < need || ((uintptr_t)d_ws & 15))) SCORE_REFUSE(c, "mica_distill_loss", "workspace too small or misaligned");
+    DeviceGuard guard;
+    MICA_ENTER(c);
+    launch_distill_loss(v, rows, d, temperature, d_loss, d_aux, d_ws, (hipStream_t)stream);
+    CHECK_LAUNCHES(c);
+    return MICA_OK;
+}
+
+int mica_distill_backward(mica_ctx* c, const mica_logits* z, const mica_top_list* list, float temperature, const float* d_aux, const float* d_g_loss,
+                          void* d_grad, void* stream) {
+    if (!c) return MICA_ERR_ARG;
+    LogitsView v;
+    DistillList d;
+    int64_t rows = 0;
+    if (const char* why = logits_view(z, v, rows)) SCORE_REFUSE(c, "mica_distill_backward", why);
+    if (const char* why = top_list(list, rows, d)) SCORE_REFUSE(c, "mica_distill_backward", why);
+    if (bad_temperature(temperature)) SCORE_REFUSE(c, "mica_distill_backward", "temperature must be in [1e-4, 1e4]");
+    if (!rows) return MICA_OK;
+    if (!d_g_loss || !d_grad || (!d_aux && !score_is_col(v))) SCORE_REFUSE(c, "mica_distill_backward", "null pointer");
+    DeviceGuard guard;
+    MICA_ENTER(c);
+    launch_distill_grad(v, rows, d, temperature, d_aux, d_g_loss, d_grad, (hipStream_t)stream);
+    CHECK_LAUNCHES(c);
+    return MICA_OK;
+}
+
+int mica_distill_step(mica_ctx* c, const mica_logits* z, const mica_top_list* list, float temperature, const float* d_weight, float* d_loss, void* d_grad,
+                      void* d_ws, int64_t ws_bytes, void* stream) {
+    if (!c) return MICA_ERR_ARG;
+    LogitsView v;
+    DistillList d;
+    int64_t rows = 0;
+    if (const char* why = logits_view(z, v, rows)) SCORE_REFUSE(c, "mica_distill_step", why);
+    if (const char* why = top_list(list, rows, d)) SCORE_REFUSE(c, "mica_distill_step", why);
+    if (bad_temperature(temperature)) SCORE_REFUSE(c, "mica_distill_step", "temperature must be in [1e-4, 1e4]");
+    if (!rows) return MICA_OK;
+    if (!d_loss || !d_grad) SCORE_REFUSE(c, "mica_distill_step", "null pointer");
+    const int64_t need = distill_ws_bytes(v, rows, true);
+    if (need > 0 && (!d_ws || ws_bytes < need || ((uintptr_t)d_ws & 15))) SCORE_REFUSE(c, "mica_distill_step", "workspace too small or misaligned");
+    DeviceGuard guard;
+    MICA_ENTER(c);
+    launch_distill_step(v, rows, d, temperature, d_weight, d_loss, d_grad, d_ws, (hipStream_t)stream);
+    CHECK_LAUNCHES(c);
+    return MICA_OK;
 }
 
 }  // extern "C"

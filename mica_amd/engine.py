@@ -11,6 +11,7 @@ import numpy as np
 import torch
 
 from . import _cabi
+from . import scoring
 from ._cabi import MicaHipError, AF_NONE, AF_PER_TILE, AF_BATCH, AF_ALWAYS  # noqa: F401
 
 
@@ -371,6 +372,123 @@ class Engine:
         self._check(self.lib.mica_neighbour_matrix_np(self._h, _ptr(cands), n, _ptr(bb), *bb.shape, int(bool(numpy_legacy)), _ptr(dis),
                                                       _ptr(mat), self._stream()), "mica_neighbour_matrix")
         return dis, mat
+
+    # -- scoring of class distributions, distillation from top alternatives (mica_amd/scoring.py: the differentiable forms) --------
+    def _logits(self, logits, dim, name="logits"):
+        if not isinstance(logits, torch.Tensor) or logits.device != self.device:
+            raise MicaHipError(f"{name}: expected a tensor on {self.device}, got {getattr(logits, 'device', type(logits))}")
+        return scoring.LogitsLayout(logits, dim)
+
+    def _workspace(self, nbytes):
+        """A workspace of one call, from torch's allocator: its stream and graph rules hold for it."""
+        if nbytes < 0:
+            raise MicaHipError(f"workspace query refused ({nbytes})")
+        return torch.empty((nbytes,), dtype=torch.uint8, device=self.device) if nbytes else None
+
+    def _f32_rows(self, shape):
+        return torch.empty(shape, dtype=torch.float32, device=self.device)
+
+    def token_logprobs(self, logits: torch.Tensor, tokens: torch.Tensor | None = None, top: int = 0, dim: int = -1, temperature: float = 1.0,
+                       ignore_index: int = -100):
+        """Scores of the distributions softmax(logits / temperature) along `dim` -> scoring.TokenScores:
+        logprob (of `tokens`, integers of the logits' shape without `dim`; ignore_index: 0, any other value outside [0, classes): NaN),
+        entropy and lse (log sum exp), all float32; top_logprob float32 / top_index int32, the `top` (<= 64) most probable classes in
+        order, ties to the lowest class.  Logits float32, bfloat16 or float16 of any strides.  A row whose classes are all -inf: log
+        probabilities -inf, entropy 0.  Asynchronous; the results have no autograd history (scoring.token_logprobs has)."""
+        v = self._logits(logits, dim)
+        temperature = scoring.check_temperature(temperature)
+        top = int(top)
+        if not 0 <= top <= min(scoring.MAX_TOP, v.classes):
+            raise MicaHipError(f"top must be in [0, {min(scoring.MAX_TOP, v.classes)}], got {top}")
+        logprob = topv = topi = None
+        if tokens is not None:
+            tokens = scoring.check_ints(tokens, "tokens", v.rows_shape, self.device).contiguous()
+            logprob = self._f32_rows(v.rows_shape)
+        entropy, lse = self._f32_rows(v.rows_shape), self._f32_rows(v.rows_shape)
+        if top:
+            topv = self._f32_rows(v.with_axis(top))
+            topi = torch.empty(v.with_axis(top), dtype=torch.int32, device=self.device)
+        if v.rows:
+            ws = self._workspace(self.lib.mica_token_logprobs_ws(C.byref(v.desc), top))
+            self._check(self.lib.mica_token_logprobs(
+                self._h, C.byref(v.desc), _ptr(tokens), 0 if tokens is None else tokens.element_size(), int(ignore_index), temperature, top,
+                _ptr(logprob), _ptr(entropy), _ptr(lse), _ptr(topv), _ptr(topi), _ptr(ws), 0 if ws is None else ws.numel(), self._stream()),
+                "mica_token_logprobs")
+        return scoring.TokenScores(logprob, entropy, lse, None if topv is None else v.give(topv), None if topi is None else v.give(topi))
+
+    def token_logprobs_backward(self, logits, tokens, lse, entropy, g_logprob=None, g_entropy=None, g_lse=None, dim: int = -1,
+                                temperature: float = 1.0, ignore_index: int = -100) -> torch.Tensor:
+        """Gradient, in the logits' type and shape, of (g_logprob logprob + g_entropy entropy + g_lse lse).sum(); lse and entropy are
+        token_logprobs' results for the same logits and temperature; each upstream gradient may be None."""
+        v = self._logits(logits, dim)
+        temperature = scoring.check_temperature(temperature)
+        rows = []
+        for t, name in ((lse, "lse"), (entropy, "entropy"), (g_logprob, "g_logprob"), (g_entropy, "g_entropy"), (g_lse, "g_lse")):
+            if t is None and name.startswith("g_"):
+                rows.append(None)
+            else:
+                rows.append(scoring.check_floats(t, name, v.rows_shape, self.device).contiguous())
+        if g_logprob is not None:
+            tokens = scoring.check_ints(tokens, "tokens", v.rows_shape, self.device).contiguous()
+        else:
+            tokens = None
+        grad = torch.empty(v.with_axis(v.classes), dtype=logits.dtype, device=self.device)
+        if v.rows:
+            self._check(self.lib.mica_token_logprobs_backward(
+                self._h, C.byref(v.desc), _ptr(tokens), 0 if tokens is None else tokens.element_size(), int(ignore_index), temperature,
+                *[_ptr(t) for t in rows], _ptr(grad), self._stream()), "mica_token_logprobs_backward")
+        return v.give(grad)
+
+    def distill_loss(self, student: torch.Tensor, teacher_index: torch.Tensor, teacher_logprob: torch.Tensor, dim: int = -1,
+                     temperature: float = 1.0, tail: bool = False):
+        """Kullback-Leibler divergence, times temperature^2, of softmax(student / temperature) from a teacher known by its K (<= 256)
+        top alternatives per row -> (loss float32, rows; aux for distill_backward).
+        teacher_index (int32 / int64, negative = unused entry) and teacher_logprob (log probabilities at the same temperature, e.g.
+        token_logprobs(teacher, top=K, temperature=T)) have K at axis `dim`.  tail=False: the list is renormalised over its K entries;
+        tail=True: all classes not listed share the teacher's remaining mass 1 - sum p as one alternative.  A row without used entries
+        has loss 0; a student row of -inf only: loss +inf, gradient 0; an index >= classes: NaN."""
+        v = self._logits(student, dim, "student")
+        temperature = scoring.check_temperature(temperature)
+        lst, keep = scoring.top_list(v, teacher_index, teacher_logprob, tail, self.device)
+        loss = self._f32_rows(v.rows_shape)
+        aux = self._f32_rows((4, v.rows) if v.classes > scoring.COL_MAX else (0,))
+        if v.rows:
+            ws = self._workspace(self.lib.mica_distill_ws(C.byref(v.desc), 0))
+            self._check(self.lib.mica_distill_loss(self._h, C.byref(v.desc), C.byref(lst), temperature, _ptr(loss), _ptr(aux) if aux.numel() else None,
+                                                   _ptr(ws), 0 if ws is None else ws.numel(), self._stream()), "mica_distill_loss")
+        del keep
+        return loss, aux
+
+    def distill_backward(self, student, teacher_index, teacher_logprob, aux, g_loss, dim: int = -1, temperature: float = 1.0, tail: bool = False):
+        """Gradient, in the student's type and shape, of (g_loss * loss).sum(); aux: distill_loss' second result for the same arguments."""
+        v = self._logits(student, dim, "student")
+        temperature = scoring.check_temperature(temperature)
+        lst, keep = scoring.top_list(v, teacher_index, teacher_logprob, tail, self.device)
+        aux = scoring.check_floats(aux, "aux", (4, v.rows) if v.classes > scoring.COL_MAX else (0,), self.device).contiguous()
+        g_loss = scoring.check_floats(g_loss, "g_loss", v.rows_shape, self.device).contiguous()
+        grad = torch.empty(v.with_axis(v.classes), dtype=student.dtype, device=self.device)
+        if v.rows:
+            self._check(self.lib.mica_distill_backward(self._h, C.byref(v.desc), C.byref(lst), temperature, _ptr(aux) if aux.numel() else None,
+                                                       _ptr(g_loss), _ptr(grad), self._stream()), "mica_distill_backward")
+        del keep
+        return v.give(grad)
+
+    def distill_step(self, student, teacher_index, teacher_logprob, dim: int = -1, temperature: float = 1.0, tail: bool = False, weight=None):
+        """The training step's form: (weight * loss, gradient of its sum with respect to the student's logits) in one call.  weight
+        float32, one per row (None: 1); rows of weight 0 give loss 0 and gradient 0 whatever they hold."""
+        v = self._logits(student, dim, "student")
+        temperature = scoring.check_temperature(temperature)
+        lst, keep = scoring.top_list(v, teacher_index, teacher_logprob, tail, self.device)
+        if weight is not None:
+            weight = scoring.check_floats(weight, "weight", v.rows_shape, self.device).contiguous()
+        loss = self._f32_rows(v.rows_shape)
+        grad = torch.empty(v.with_axis(v.classes), dtype=student.dtype, device=self.device)
+        if v.rows:
+            ws = self._workspace(self.lib.mica_distill_ws(C.byref(v.desc), 1))
+            self._check(self.lib.mica_distill_step(self._h, C.byref(v.desc), C.byref(lst), temperature, _ptr(weight), _ptr(loss), _ptr(grad), _ptr(ws),
+                                                   0 if ws is None else ws.numel(), self._stream()), "mica_distill_step")
+        del keep
+        return loss, v.give(grad)
 
     # -- single ops (tests) -----------------------------------------------------------------------------
     def op_conv3d(self, x, w, b, k, variant: int = 0):

@@ -82,4 +82,12 @@ class MICA:
         af = None if af_features is None else af_features.to(dev, torch.float32)
         return e.forward_logits(exp_map.to(dev, torch.float32), af, AF_BATCH)
 
+    def amino_acid_scores(self, exp_map: torch.Tensor, af_features: torch.Tensor | None = None, residues: torch.Tensor | None = None, top: int = 3,
+                          temperature: float = 1.0):
+        """forward(), then scoring.TokenScores of the amino-acid head at every voxel over the 20 residues (0..19, the background class
+        left out as utils/predict.py:348 of the reference does): log probability of `residues` (integers [B,D,H,W], -100 = none),
+        entropy, and the `top` alternatives [B,top,D,H,W] - the list a student is distilled from (scoring.distill_loss)."""
+        aa = self.forward(exp_map, af_features)[2]
+        return self._engine(exp_map.shape[2:]).token_logprobs(aa[:, 1:], residues, top=top, dim=1, temperature=temperature)
+
     __call__ = forward
