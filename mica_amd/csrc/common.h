@@ -277,7 +277,7 @@ int segment_sums_device(const float* d_vals, const int64_t* d_seg_off, int64_t n
 int nms_points_device(const int* d_pts, int64_t n, int n0, int n1, int n2, double radius, int* d_keep, hipStream_t st, char* err, int errlen);
 // class scoring and distillation (kernels_score.hip); the entry points have checked the view
 constexpr int SCORE_COL_MAX = 64;            // up to here a thread holds all classes of a row in registers
-constexpr int SCORE_SEG_MAX = 131072;        // classes one block streams (a bit per class in LDS: 16 KB)
+constexpr int SCORE_SEG_BYTES = 262144;      // of a row that one block streams (a byte of LDS marks 16 of them)
 struct LogitsView { const void* p; int dtype, class_last; int64_t outer, inner, classes, so, si, sc; };
 struct DistillList { const void* index; const void* teacher; int index_bytes, teacher_dtype, k, tail; };
 struct SegPlan { int n, len; };              // a row is cut into n segments of len classes

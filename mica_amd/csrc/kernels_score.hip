@@ -60,6 +60,25 @@ __device__ __forceinline__ void unpack(uint4v q, float (&f)[8], f16_t*) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) f[j] = (float)h[j];
 }
+// the elements of a raw vector that b names become -inf
+__device__ __forceinline__ uint4v raw_drop(uint4v q, unsigned b, float*) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) q[j] = (b >> j) & 1u ? 0xFF800000u : q[j];
+    return q;
+}
+template <typename T> __device__ __forceinline__ uint4v raw_drop(uint4v q, unsigned b, T*) {
+    constexpr unsigned inf = std::is_same<T, bf16_t>::value ? 0xFF80u : 0xFC00u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        q[j] = (b >> (2 * j)) & 1u ? (q[j] & 0xFFFF0000u) | inf : q[j];
+        q[j] = (b >> (2 * j + 1)) & 1u ? (q[j] & 0xFFFFu) | (inf << 16) : q[j];
+    }
+    return q;
+}
+template <typename T> __device__ __forceinline__ uint4v raw_neg_inf();
+template <> __device__ __forceinline__ uint4v raw_neg_inf<float>() { return 0xFF800000u; }
+template <> __device__ __forceinline__ uint4v raw_neg_inf<bf16_t>() { return 0xFF80FF80u; }
+template <> __device__ __forceinline__ uint4v raw_neg_inf<f16_t>() { return 0xFC00FC00u; }
 template <typename T, int N> __device__ __forceinline__ void store_vec(T* p, const float (&f)[N]) {
     struct alignas(16) { T t[N]; } o;
 #pragma unroll
@@ -81,109 +100,179 @@ __device__ __forceinline__ float key_value(unsigned k) {
 __device__ __forceinline__ u64 make_key(unsigned o, unsigned index) { return ((u64)o << 32) | (0xFFFFFFFFu - index); }
 __device__ __forceinline__ unsigned key_index(u64 k) { return 0xFFFFFFFFu - (unsigned)k; }
 
-// ---- reductions over a wave ---------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
+// ---- exchange between the lanes of a wave, on the vector ALU (no LDS round trip) ---------------------------------------------------------
+template <int CTRL> __device__ __forceinline__ unsigned dpp(unsigned v) { return __builtin_amdgcn_update_dpp(0u, v, CTRL, 0xF, 0xF, true); }
+// the value of lane ^ O
+template <int O> __device__ __forceinline__ unsigned lane_xor(unsigned v) {
+    if constexpr (O == 1) return dpp<0xB1>(v);                       // quad_perm 1 0 3 2
+    else if constexpr (O == 2) return dpp<0x4E>(v);                  // quad_perm 2 3 0 1
+    else if constexpr (O == 4) return dpp<0x1B>(dpp<0x141>(v));      // half-row mirror (^ 7), quad_perm 3 2 1 0 (^ 3)
+    else if constexpr (O == 8) return dpp<0x128>(v);                 // row rotate by 8
+    else if constexpr (O == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        return (threadIdx.x & 16) ? r[0] : r[1];
+    } else {
+        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        return (threadIdx.x & 32) ? r[0] : r[1];
+    }
 }
-template <typename F> __device__ __forceinline__ F wave_sum(F v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    return v;
+template <int O> __device__ __forceinline__ float lane_xor(float v) { return __builtin_bit_cast(float, lane_xor<O>(__builtin_bit_cast(unsigned, v))); }
+template <int O> __device__ __forceinline__ u64 lane_xor(u64 v) { return ((u64)lane_xor<O>((unsigned)(v >> 32)) << 32) | lane_xor<O>((unsigned)v); }
+template <int O> __device__ __forceinline__ double lane_xor(double v) { return __builtin_bit_cast(double, lane_xor<O>(__builtin_bit_cast(u64, v))); }
+
+template <typename F, typename Op> __device__ __forceinline__ F wave_all(F v, Op op) {      // the same value in every lane
+    v = op(v, lane_xor<1>(v));
+    v = op(v, lane_xor<2>(v));
+    v = op(v, lane_xor<4>(v));
+    v = op(v, lane_xor<8>(v));
+    v = op(v, lane_xor<16>(v));
+    return op(v, lane_xor<32>(v));
 }
-__device__ __forceinline__ void wave_sync() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+__device__ __forceinline__ float wave_max(float v) { return wave_all(v, [](float a, float b) { return fmaxf(a, b); }); }
+template <typename F> __device__ __forceinline__ F wave_sum(F v) { return wave_all(v, [](F a, F b) { return a + b; }); }
+
+__device__ __forceinline__ void wave_sync() {                       // LDS written by some lanes of a wave, read by others
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
     __builtin_amdgcn_wave_barrier();
 }
 template <int G> __device__ __forceinline__ void group_sync() {
-    if (G == 64) { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup"); __builtin_amdgcn_wave_barrier(); }
+    if (G == 64) wave_sync();
     else __syncthreads();
-}
-// over a group of G threads: a wave, or the whole block (`red`: one double per wave of the block)
-template <int G> __device__ __forceinline__ float group_max(float v, double* red) {
-    v = wave_max(v);
-    if (G > 64) {
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-        __syncthreads();
-        v = (float)red[0];
-#pragma unroll
-        for (int i = 1; i < G / 64; ++i) v = fmaxf(v, (float)red[i]);
-    }
-    return v;
-}
-template <int G> __device__ __forceinline__ double group_sum(double v, double* red) {
-    v = wave_sum(v);
-    if (G > 64) {
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-        __syncthreads();
-        v = 0.0;
-#pragma unroll
-        for (int i = 0; i < G / 64; ++i) v += red[i];
-    }
-    return v;
 }
 
 // ---- the 64 largest keys of a wave: one per lane, descending ------------------------------------------------------------------------
-__device__ __forceinline__ u64 shfl_xor64(u64 v, int o) {
-    const unsigned lo = __shfl_xor((unsigned)v, o), hi = __shfl_xor((unsigned)(v >> 32), o);
-    return ((u64)hi << 32) | lo;
-}
-__device__ __forceinline__ u64 shfl64(u64 v, int l) {
-    const unsigned lo = __shfl((unsigned)v, l), hi = __shfl((unsigned)(v >> 32), l);
-    return ((u64)hi << 32) | lo;
-}
-__device__ __forceinline__ u64 cmp_exchange(u64 v, int o, bool take_max) {
-    const u64 w = shfl_xor64(v, o);
+template <int O> __device__ __forceinline__ u64 cmp_exchange(u64 v, bool take_max) {
+    const u64 w = lane_xor<O>(v);
     return (v > w) == take_max ? v : w;
 }
-__device__ __forceinline__ u64 bitonic_merge64(u64 v, int lane) {      // a bitonic sequence -> descending
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = cmp_exchange(v, o, (lane & o) == 0);
-    return v;
+// a bitonic sequence -> descending, or ascending
+template <bool DESC> __device__ __forceinline__ u64 bitonic_merge64(u64 v, int lane) {
+    v = cmp_exchange<32>(v, ((lane & 32) == 0) == DESC);
+    v = cmp_exchange<16>(v, ((lane & 16) == 0) == DESC);
+    v = cmp_exchange<8>(v, ((lane & 8) == 0) == DESC);
+    v = cmp_exchange<4>(v, ((lane & 4) == 0) == DESC);
+    v = cmp_exchange<2>(v, ((lane & 2) == 0) == DESC);
+    return cmp_exchange<1>(v, ((lane & 1) == 0) == DESC);
 }
-__device__ __forceinline__ u64 sort64(u64 v, int lane) {               // descending
-#pragma unroll
-    for (int k = 2; k < 64; k <<= 1)
-#pragma unroll
-        for (int o = k >> 1; o > 0; o >>= 1) v = cmp_exchange(v, o, ((lane & o) == 0) == ((lane & k) == 0));
-    return bitonic_merge64(v, lane);
+template <bool DESC> __device__ __forceinline__ u64 sort64(u64 v, int lane) {
+#define MICA_SORT_STEP(k, o) v = cmp_exchange<o>(v, ((lane & (o)) == 0) == ((lane & (k)) == 0))
+    MICA_SORT_STEP(2, 1);
+    MICA_SORT_STEP(4, 2); MICA_SORT_STEP(4, 1);
+    MICA_SORT_STEP(8, 4); MICA_SORT_STEP(8, 2); MICA_SORT_STEP(8, 1);
+    MICA_SORT_STEP(16, 8); MICA_SORT_STEP(16, 4); MICA_SORT_STEP(16, 2); MICA_SORT_STEP(16, 1);
+    MICA_SORT_STEP(32, 16); MICA_SORT_STEP(32, 8); MICA_SORT_STEP(32, 4); MICA_SORT_STEP(32, 2); MICA_SORT_STEP(32, 1);
+#undef MICA_SORT_STEP
+    return bitonic_merge64<DESC>(v, lane);
 }
-// a, b descending, b given reversed (lane i holds the (63 - i)-th): the 64 largest of both, descending
-__device__ __forceinline__ u64 merge_top64(u64 a, u64 b_reversed, int lane) { return bitonic_merge64(a > b_reversed ? a : b_reversed, lane); }
+// a descending, b ascending: the 64 largest of both, descending
+__device__ __forceinline__ u64 merge_top64(u64 a, u64 b, int lane) { return bitonic_merge64<true>(a > b ? a : b, lane); }
+__device__ __forceinline__ u64 lane_key(u64 v, int l) {             // of a lane known to all
+    const unsigned lo = __builtin_amdgcn_readlane((unsigned)v, l), hi = __builtin_amdgcn_readlane((unsigned)(v >> 32), l);
+    return ((u64)hi << 32) | lo;
+}
 
 // ---- online softmax of one thread -----------------------------------------------------------------------------------------------------
-// m: running maximum, s = sum 2^{(z - m) c}, w = sum 2^{(z - m) c} (z - m) c.  Differences to the maximum, not z c - m c: a row of the
-// type's lowest values would overflow there.
+// m: running maximum;  s = sum 2^{z c - R}, w = sum 2^{z c - R} (z c - R) with the reference R = m c rounded to float32.  One fma per
+// logit, and R being off by a rounding cancels: whoever reads s uses the same R (reference(), log_sum()).  Beyond |m| = BIG, where m c
+// may overflow (a row of the type's lowest values), the sums are relative to m c itself and the exponents (z - m) c.
+constexpr float BIG = 1.0e30f;
+__device__ __forceinline__ float reference(float m, float c) {
+#pragma clang fp contract(off)
+    return m * c;
+}
+// exponent between the references of two maxima, old <= now; -inf - -inf and the like end at NEG_BIG (with empty sums)
+__device__ __forceinline__ float ref_step(float old, float now, float c) {
+#pragma clang fp contract(off)
+    const float d = !(fabsf(old) <= BIG) || !(fabsf(now) <= BIG) ? (old - now) * c : reference(old, c) - reference(now, c);
+    return fmaxf(d, NEG_BIG);
+}
+// log of sum_v e^{(z_v - m) / T}; -inf for an empty row
+__device__ __forceinline__ double log_sum(float m, double s, float c) {
+    const double l = log(s);
+    return fabsf(m) <= BIG ? l + ((double)reference(m, c) - (double)m * c) * LN2 : l;
+}
 struct Online {
     float m = -INFINITY, s = 0.f, w = 0.f;
+    // to a maximum >= m
+    __device__ __forceinline__ void rescale(float mn, float c) {
+        const float d = ref_step(m, mn, c), a = exp2_hw(d);
+        if (m == -INFINITY) {                                // nothing so far, or NaN only
+            w = s;
+        } else {
+            w = a * fmaf(s, d, w);
+            s *= a;
+        }
+        m = mn;
+    }
+    __device__ __forceinline__ void join(Online b, float c) {
+        const float mn = fmaxf(m, b.m);
+        rescale(mn, c);
+        b.rescale(mn, c);
+        s += b.s;
+        w += b.w;
+    }
+    // N logits, vmax their maximum (never NaN).  All lanes of a wave call it together.
     template <int N, bool ENT> __device__ __forceinline__ void add(const float (&f)[N], float vmax, float c) {
         const float mn = fmaxf(m, vmax);
-        const float d = fmaxf((m - mn) * c, NEG_BIG);         // -inf - -inf = NaN -> NEG_BIG, with s = w = 0
+        if (__builtin_expect(__any(!(fabsf(mn) <= BIG)), 0)) {       // some lane's maximum is -inf, or beyond BIG
+            rescale(mn, c);
+            const bool far = !(fabsf(mn) <= BIG) && mn != -INFINITY;
+            const float R = far || mn == -INFINITY ? 0.f : reference(mn, c), sub = far ? mn : 0.f;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const float x = far ? (f[j] - sub) * c : fmaf(f[j], c, -R);
+                const float e = exp2_hw(x);
+                s += e;
+                if (ENT) w = fmaf(e, fmaxf(x, NEG_BIG), w);
+            }
+            return;
+        }
+        const float R = reference(mn, c);
+        const float d = fmaxf(reference(m, c) - R, NEG_BIG);
         const float a = exp2_hw(d);
         if (ENT) w = a * fmaf(s, d, w);
         s *= a;
         m = mn;
-        const float ref = mn == -INFINITY ? 0.f : mn;
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            const float x = (f[j] - ref) * c;
+            const float x = fmaf(f[j], c, -R);
             const float e = exp2_hw(x);
             s += e;
             if (ENT) w = fmaf(e, fmaxf(x, NEG_BIG), w);
         }
     }
-    // rescaled to a maximum >= m
-    __device__ __forceinline__ void rescale(float mn, float c) {
-        const float d = fmaxf((m - mn) * c, NEG_BIG);
-        const float a = m == -INFINITY ? 0.f : exp2_hw(d);
-        w = m == -INFINITY && s == 0.f ? 0.f : a * fmaf(s, d, w);
-        s = m == -INFINITY && s == 0.f ? 0.f : (m == -INFINITY ? s : s * a);      // a NaN row keeps its NaN
-        m = mn;
-    }
 };
+// the joined sums of a wave, in every lane
+__device__ __forceinline__ Online wave_join(Online o, float c) {
+    o.rescale(wave_max(o.m), c);
+    o.s = wave_sum(o.s);
+    o.w = wave_sum(o.w);
+    return o;
+}
+struct Partial { float m, s, w, unused; };                 // of a wave, or of a segment of a row
+// the joined sums of a group, in every thread (`part`: one entry per wave of the block)
+template <int G> __device__ __forceinline__ Online group_join(Online o, float c, Partial* part) {
+    o = wave_join(o, c);
+    if (G > 64) {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = {o.m, o.s, o.w, 0.f};
+        __syncthreads();
+        float m = part[0].m;
+#pragma unroll
+        for (int i = 1; i < G / 64; ++i) m = fmaxf(m, part[i].m);
+        o = Online();
+        o.m = m;
+#pragma unroll
+        for (int i = 0; i < G / 64; ++i) {
+            Online b;
+            b.m = part[i].m; b.s = part[i].s; b.w = part[i].w;
+            b.rescale(m, c);
+            o.s += b.s;
+            o.w += b.w;
+        }
+    }
+    return o;
+}
 
 template <int N> __device__ __forceinline__ float max_of(const float (&f)[N]) {
     float v = -INFINITY;                                       // never NaN
@@ -219,32 +308,35 @@ __device__ __forceinline__ ListPos list_pos(const LogitsView& v, RowPos p, int64
 // ========================================================================================================================================
 constexpr int UNROLL = 4;
 
-// Streams the n classes at z: f(values[N], first index) for every 16-byte vector of this thread, values beyond n = -inf.
-template <typename T, int G, typename F> __device__ __forceinline__ void stream_row(const T* __restrict__ z, int n, int tid, F&& f) {
+// Streams the n classes at z: f(raw[UNROLL], i) for UNROLL 16-byte vectors of this thread at a time (vector i + u G is the u-th), with the
+// next ones on their way; then g(values[N], vector) for each vector of the rest, classes beyond n = -inf.  All threads of the group make
+// the same calls, g also for vectors that lie beyond n.
+template <typename T, int G, typename F, typename H> __device__ __forceinline__ void stream_row(const T* __restrict__ z, int n, int tid, F&& f, H&& g) {
     constexpr int N = Vec<T>::N;
-    const int nfull = n / N;
-    int i = tid;
-    for (; i + (UNROLL - 1) * G < nfull; i += UNROLL * G) {
+    const int nfull = n / N, rounds = nfull / (UNROLL * G);
+    if (rounds > 0) {
         uint4v q[UNROLL];
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) q[u] = load_raw(z + (int64_t)(i + u * G) * N);
+        for (int u = 0; u < UNROLL; ++u) q[u] = load_raw(z + (int64_t)(tid + u * G) * N);
+        for (int it = 1; it < rounds; ++it) {
+            uint4v next[UNROLL];
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            float v[N];
-            unpack(q[u], v, (T*)nullptr);
-            f(v, (i + u * G) * N);
+            for (int u = 0; u < UNROLL; ++u) next[u] = load_raw(z + (int64_t)(tid + (it * UNROLL + u) * G) * N);
+            f(q, tid + (it - 1) * UNROLL * G);
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) q[u] = next[u];
         }
+        f(q, tid + (rounds - 1) * UNROLL * G);
     }
-    for (; i < nfull; i += G) {
+    for (int i = rounds * UNROLL * G; i * N < n; i += G) {
+        const int vec = i + tid;
         float v[N];
-        unpack(load_raw(z + (int64_t)i * N), v, (T*)nullptr);
-        f(v, i * N);
-    }
-    if (i == nfull && nfull * N < n) {
-        float v[N];
+        if (vec < nfull) unpack(load_raw(z + (int64_t)vec * N), v, (T*)nullptr);
+        else {
 #pragma unroll
-        for (int j = 0; j < N; ++j) v[j] = nfull * N + j < n ? to_f32(z[nfull * N + j]) : -INFINITY;
-        f(v, nfull * N);
+            for (int j = 0; j < N; ++j) v[j] = vec * N + j < n ? to_f32(z[vec * N + j]) : -INFINITY;
+        }
+        g(v, vec);
     }
 }
 
@@ -256,26 +348,30 @@ struct TopScratch {             // LDS of one wave
     u64 list[64];
     u64 buf[128];
 };
+// the merged top 64 of the block's waves; `list` descending per wave
+template <int NW> __device__ __forceinline__ u64 merge_waves(u64 list, TopScratch* sc, int w, int lane) {
+    sc[w].list[lane] = list;
+    __syncthreads();
+    list = sc[0].list[lane];
+#pragma unroll
+    for (int i = 1; i < NW; ++i) list = merge_top64(list, sc[i].list[63 - lane], lane);
+    return list;
+}
 template <typename T, int G>
 __device__ __forceinline__ u64 group_top(const T* __restrict__ z, int n, unsigned index0, int k, float best, int best_at, bool any, TopScratch* sc,
                                          int* owners, int* nown) {
     constexpr int N = Vec<T>::N, NW = G / 64;
     const int tid = G == 64 ? (threadIdx.x & 63) : threadIdx.x, lane = threadIdx.x & 63, w = G == 64 ? 0 : threadIdx.x >> 6;
     const u64 mine = any ? make_key(order_key(best), (unsigned)best_at) : 0;
-    u64 sorted = sort64(mine, lane);
+    u64 sorted = sort64<true>(mine, lane);
     if (NW > 1) {
-        sc[w].list[lane] = sorted;
         if (threadIdx.x == 0) *nown = 0;
-        __syncthreads();
-        sorted = sc[0].list[lane];
-#pragma unroll
-        for (int i = 1; i < NW; ++i) sorted = merge_top64(sorted, sc[i].list[63 - lane], lane);
+        sorted = merge_waves<NW>(sorted, sc, w, lane);
     }
-    const u64 bound = shfl64(sorted, k - 1);
+    const u64 bound = lane_key(sorted, k - 1);
     int count;
     if (NW > 1) {
-        const bool own = any && mine >= bound;
-        if (own) owners[atomicAdd(nown, 1)] = tid;      // the order of the owners does not change the result
+        if (any && mine >= bound) owners[atomicAdd(nown, 1)] = tid;      // the order of the owners does not change the result
         __syncthreads();
         count = *nown;
     } else {
@@ -285,12 +381,12 @@ __device__ __forceinline__ u64 group_top(const T* __restrict__ z, int n, unsigne
         count = __popcll(b);
     }
     const int nvec = (n + N - 1) / N, per = (nvec + G - 1) / G;
-    const int64_t total = (int64_t)count * per;
+    const int total = count * per;
     u64 list = 0, floor_key = 0;
     int pending = 0;
-    for (int64_t p0 = 0; p0 < total; p0 += G) {
-        const int64_t p = p0 + tid;
-        const int vec = p < total ? owners[p % count] + (int)(p / count) * G : nvec;
+    for (int p0 = 0; p0 < total; p0 += G) {
+        const int p = p0 + tid;
+        const int vec = p < total ? owners[p % count] + (p / count) * G : nvec;
         float v[N];
         if ((vec + 1) * N <= n) unpack(load_raw(z + (int64_t)vec * N), v, (T*)nullptr);
         else {
@@ -314,23 +410,15 @@ __device__ __forceinline__ u64 group_top(const T* __restrict__ z, int n, unsigne
                 sc[w].buf[lane] = rest;
                 wave_sync();
                 pending -= 64;
-                const u64 s = sort64(take, lane);
-                list = merge_top64(list, shfl64(s, 63 - lane), lane);
-                floor_key = shfl64(list, k - 1);
+                list = merge_top64(list, sort64<false>(take, lane), lane);
+                floor_key = lane_key(list, k - 1);
             }
         }
     }
-    if (pending > 0) {
-        const u64 s = sort64(lane < pending ? sc[w].buf[lane] : 0, lane);
-        list = merge_top64(list, shfl64(s, 63 - lane), lane);
-    }
+    if (pending > 0) list = merge_top64(list, sort64<false>(lane < pending ? sc[w].buf[lane] : 0, lane), lane);
     if (NW > 1) {
         __syncthreads();
-        sc[w].list[lane] = list;
-        __syncthreads();
-        list = sc[0].list[lane];
-#pragma unroll
-        for (int i = 1; i < NW; ++i) list = merge_top64(list, sc[i].list[63 - lane], lane);
+        list = merge_waves<NW>(list, sc, w, lane);
     }
     // classes are numbered within the segment so far
     return list == 0 ? 0 : ((list & 0xFFFFFFFF00000000ull) | (0xFFFFFFFFu - (key_index(list) + index0)));
@@ -349,41 +437,41 @@ struct ScoreOut {
     int top;
     float c, inv_t;
 };
-// natural logarithm of the sum relative to the maximum
-__device__ __forceinline__ float row_lse(float m, float log_s, float inv_t) { return m == -INFINITY ? -INFINITY : (float)((double)m * inv_t + log_s); }
-__device__ __forceinline__ float class_logprob(float z, float m, float log_s, float inv_t) {
-    return m == -INFINITY ? (log_s != log_s ? log_s : -INFINITY) : (float)((double)(z - m) * inv_t - log_s);
+// L: the type the row's scalars are combined in
+template <typename L> __device__ __forceinline__ float class_logprob(float z, float m, L log_s, float inv_t) {
+    const float lp = m == -INFINITY ? (log_s != log_s ? (float)log_s : -INFINITY) : (float)((L)(z - m) * inv_t - log_s);
+    return lp > 0.f ? 0.f : lp;                                 // a sum that rounded to just below 1
 }
-template <typename T>
-__device__ __forceinline__ void write_row(const ScoreOut& o, const T* __restrict__ z, int64_t sc, int64_t classes, int64_t r, float m, float s, float w) {
-    const float log_s = (float)log((double)s);            // s >= 1 unless the row is empty (0) or holds NaN
-    o.lse[r] = s != s ? s : row_lse(m, log_s, o.inv_t);
-    o.entropy[r] = s == 0.f ? 0.f : (float)(LN2 * (log2((double)s) - (double)w / s));
+template <typename T, typename L>
+__device__ __forceinline__ void write_row(const ScoreOut& o, const T* __restrict__ z, int64_t sc, int64_t classes, int64_t r, float m, float s, float w,
+                                          L log_s) {
+    o.lse[r] = s != s ? s : (m == -INFINITY ? -INFINITY : (float)((L)m * o.inv_t + log_s));
+    // log2 s - w / s in the units of R cancels nothing: both parts of the entropy are >= 0 up to rounding
+    const L log2_s = sizeof(L) == 8 ? (L)log2((double)s) : (L)log2f(s);
+    const float h = s == 0.f ? 0.f : (float)((L)LN2 * (log2_s - (L)w / (L)s));
+    o.entropy[r] = h < 0.f ? 0.f : h;
     if (o.logprob) {
         const int64_t t = load_int(o.tokens, r, o.token_bytes);
         float lp;
         if (t == o.ignore) lp = 0.f;
         else if (t < 0 || t >= classes) lp = NAN;
-        else lp = s != s ? s : class_logprob(to_f32(z[t * sc]), m, log_s, o.inv_t);
+        else lp = s != s ? s : class_logprob<L>(to_f32(z[t * sc]), m, log_s, o.inv_t);
         o.logprob[r] = lp;
     }
 }
-__device__ __forceinline__ void write_top(const ScoreOut& o, const LogitsView& v, RowPos p, int64_t r, u64 key, int lane, float m, float s) {
+__device__ __forceinline__ void write_top(const ScoreOut& o, const LogitsView& v, RowPos p, int64_t r, u64 key, int lane, float m, float s, double log_s) {
     if (lane < o.top) {
-        const float log_s = (float)log((double)s);
         const ListPos l = list_pos(v, p, r, o.top);
-        o.top_logprob[l.base + lane * l.stride] = s != s ? s : class_logprob(key_value((unsigned)(key >> 32)), m, log_s, o.inv_t);
+        o.top_logprob[l.base + lane * l.stride] = s != s ? s : class_logprob<double>(key_value((unsigned)(key >> 32)), m, log_s, o.inv_t);
         o.top_index[l.base + lane * l.stride] = (int)key_index(key);
     }
 }
 
-struct Partial { float m, s, w, unused; };                 // of one segment of a row
-
 template <typename T, int G, bool TOP>
 __global__ __launch_bounds__(256) void score_row_kernel(LogitsView v, int64_t rows, ScoreOut o, int segments, int seg_len, Partial* __restrict__ part,
                                                         u64* __restrict__ part_top) {
-    constexpr int NW = G / 64, GROUPS = 256 / G;
-    __shared__ double red[4];
+    constexpr int N = Vec<T>::N, NW = G / 64, GROUPS = 256 / G;
+    __shared__ Partial waves[4];
     __shared__ TopScratch top_sc[TOP ? 4 : 1];
     __shared__ int owners[TOP ? 256 : 1];
     __shared__ int nown;
@@ -400,67 +488,89 @@ __global__ __launch_bounds__(256) void score_row_kernel(LogitsView v, int64_t ro
     float best = -INFINITY;
     int best_at = 0;
     bool any = false;
-    stream_row<T, G>(z + first, n, tid, [&](const float(&f)[Vec<T>::N], int at) {
-        const float vm = max_of(f);
+    const auto note = [&](float vm, int vec) {
         if (TOP) {
-            if (!any || vm > best) { best = vm; best_at = at; }
+            if (vm > best || !any) { best = vm; best_at = vec * N; }
             any = true;
         }
-        on.add<Vec<T>::N, true>(f, vm, o.c);
-    });
-    const float m = group_max<G>(on.m, red);
-    on.rescale(m, o.c);
-    const float s = (float)group_sum<G>((double)on.s, red), w = (float)group_sum<G>((double)on.w, red);
+    };
+    stream_row<T, G>(
+        z + first, n, tid,
+        [&](const uint4v(&q)[UNROLL], int i) {
+            float f[UNROLL * N], vm = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) {
+                float x[N];
+                unpack(q[u], x, (T*)nullptr);
+                const float mu = max_of(x);
+                note(mu, i + u * G);
+                vm = fmaxf(vm, mu);
+#pragma unroll
+                for (int j = 0; j < N; ++j) f[u * N + j] = x[j];
+            }
+            on.add<UNROLL * N, true>(f, vm, o.c);
+        },
+        [&](const float(&f)[N], int vec) {
+            const float vm = max_of(f);
+            if (vec * N < n) note(vm, vec);
+            on.add<N, true>(f, vm, o.c);
+        });
+    on = group_join<G>(on, o.c, waves);
     u64 key = 0;
     if (TOP) key = group_top<T, G>(z + first, n, (unsigned)first, o.top, best, best_at, any, NW == 1 ? &top_sc[g] : top_sc, &owners[g * G], &nown);
     if (segments == 1) {
-        if (tid == 0) write_row<T>(o, z, 1, v.classes, r, m, s, w);
-        if (TOP && tid < 64) write_top(o, v, p, r, key, lane, m, s);
+        if (tid < 64) {
+            const double log_s = log_sum(on.m, on.s, o.c);        // s is about 1 or more unless the row is empty (0) or holds NaN
+            if (lane == 0) write_row<T, double>(o, z, 1, v.classes, r, on.m, on.s, on.w, log_s);
+            if (TOP) write_top(o, v, p, r, key, lane, on.m, on.s, log_s);
+        }
     } else {
-        if (tid == 0) part[item] = {m, s, w, 0.f};
+        if (tid == 0) part[item] = {on.m, on.s, on.w, 0.f};
         if (TOP && tid < o.top) part_top[item * 64 + tid] = key;
     }
 }
 
-// joins the segments of a row: one block of 256
+// joins the segments of a row: a block of 16 waves
+constexpr int JOIN = 1024;
+__device__ __forceinline__ Online join_segments(const Partial* __restrict__ part, int segments, float c) {      // one wave; in every lane
+    Online on;
+    for (int i = threadIdx.x & 63; i < segments; i += 64) {
+        const Partial q = part[i];
+        Online b;
+        b.m = q.m; b.s = q.s; b.w = q.w;
+        on.join(b, c);
+    }
+    return wave_join(on, c);
+}
 template <typename T, bool TOP>
-__global__ __launch_bounds__(256) void score_join_kernel(LogitsView v, ScoreOut o, int segments, const Partial* __restrict__ part,
-                                                         const u64* __restrict__ part_top) {
-    __shared__ double red[4];
-    __shared__ u64 lists[4][64];
+__global__ __launch_bounds__(TOP ? JOIN : 64) void score_join_kernel(LogitsView v, ScoreOut o, int segments, const Partial* __restrict__ part,
+                                                                     const u64* __restrict__ part_top) {
+    __shared__ u64 lists[TOP ? JOIN / 64 : 1][64];
     const int64_t r = blockIdx.x;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const RowPos p = row_pos(v, r);
     const T* z = static_cast<const T*>(v.p) + row_start(v, p);
-    Online on;
-    for (int i = threadIdx.x; i < segments; i += 256) {
-        const Partial q = part[r * segments + i];
-        Online b;
-        b.m = q.m; b.s = q.s; b.w = q.w;
-        const float mn = fmaxf(on.m, q.m);
-        on.rescale(mn, o.c);
-        b.rescale(mn, o.c);
-        on.s += b.s;
-        on.w += b.w;
-    }
-    const float m = group_max<256>(on.m, red);
-    on.rescale(m, o.c);
-    const float s = (float)group_sum<256>((double)on.s, red), ws = (float)group_sum<256>((double)on.w, red);
-    if (threadIdx.x == 0) write_row<T>(o, z, 1, v.classes, r, m, s, ws);
-    if (TOP) {
-        u64 list = 0;
-        for (int i = w; i < segments; i += 4) {
+    u64 list = 0;
+    if (TOP) {                                                      // every wave merges its share, then a tree over the waves
+        for (int i = w; i < segments; i += JOIN / 64) {
             const u64* q = part_top + (r * segments + i) * 64;
             list = merge_top64(list, 63 - lane < o.top ? q[63 - lane] : 0, lane);
         }
         lists[w][lane] = list;
-        __syncthreads();
-        if (w == 0) {
 #pragma unroll
-            for (int i = 1; i < 4; ++i) list = merge_top64(list, lists[i][63 - lane], lane);
-            write_top(o, v, p, r, list, lane, m, s);
+        for (int h = JOIN / 128; h > 0; h >>= 1) {
+            __syncthreads();
+            if (w < h) {
+                list = merge_top64(list, lists[w + h][63 - lane], lane);
+                lists[w][lane] = list;                              // read by nobody in this round: waves w + h >= h read nothing below h
+            }
         }
     }
+    if (w > (TOP ? 1 : 0)) return;
+    const Online on = join_segments(part + r * segments, segments, o.c);
+    const double log_s = log_sum(on.m, on.s, o.c);
+    if (TOP && w == 0) write_top(o, v, p, r, list, lane, on.m, on.s, log_s);
+    if (w == (TOP ? 1 : 0) && lane == 0) write_row<T, double>(o, z, 1, v.classes, r, on.m, on.s, on.w, log_s);
 }
 
 // ---- gradient of the scores ------------------------------------------------------------------------------------------------------------
@@ -568,128 +678,155 @@ struct DistillArgs {
 // A row's gradient: factor * e^{y - ref} where a class is not listed, mass * e^{y - lse} - sum p at a listed one, times T and the
 // upstream gradient.  (tail: ref is the log sum of the classes that are not listed and factor = mass q_rest - r, so that nothing
 // overflows where q_rest is tiny; else ref = lse, factor = mass.)
-struct RowDistill { float loss, ref, factor, lse, mass, norm; bool skip; };
+struct RowDistill { float loss, ref, factor, lse, mass, norm; };
 
-// dynamic LDS of a distill group: K indices, then a bit per class of the segment (tail)
-template <typename T, int G>
-__device__ __forceinline__ bool list_load(const DistillArgs& a, ListPos l, int tid, int* idx) {
-    bool used = false;
-    for (int k = tid; k < a.k; k += G) {
-        const int64_t i = load_int(a.index, l.base + k * l.stride, a.index_bytes);
-        idx[k] = i < 0 ? -1 : (i > 0x7FFFFFFE ? 0x7FFFFFFF : (int)i);
-        used |= i >= 0;
+// The row's list in LDS: index (unused entries -1, no class: INT_MAX), log probability, logit.  Loaded by one wave.
+constexpr int SLOTS = 4;                                        // entries per lane of that wave: 256 in all
+struct ListLds { int* i; float* t; float* z; };
+constexpr unsigned LIST_BYTES = 12;                             // of LDS per entry
+__device__ __forceinline__ ListLds list_lds(int* base, int k) { return {base, reinterpret_cast<float*>(base + k), reinterpret_cast<float*>(base + 2 * k)}; }
+template <typename T>
+__device__ __forceinline__ void list_load(const DistillArgs& a, ListPos l, const T* __restrict__ z, int64_t classes, int lane, ListLds d) {
+    for (int k = lane; k < a.k; k += 64) {
+        const int64_t v = load_int(a.index, l.base + k * l.stride, a.index_bytes);
+        const float t = load_float(a.teacher, l.base + k * l.stride, a.teacher_dtype);
+        d.i[k] = v < 0 ? -1 : (v >= classes ? 0x7FFFFFFF : (int)v);
+        d.t[k] = v < 0 ? -INFINITY : t;
+        d.z[k] = v < 0 || v >= classes ? -INFINITY : to_f32(z[v]);
     }
-    return used;
 }
-template <int G> __device__ __forceinline__ void mark_listed(const int* idx, int k, int first, int n, unsigned* bits, int tid) {
-    for (int i = tid; i < (n + 31) / 32; i += G) bits[i] = 0;
+// A bit per class, laid out as the stream reads it: class v of vector vec = v / N is bit (vec / G % UNROLL) * 8 + v % N of word
+// (vec / (UNROLL G)) G + vec % G, one word for the UNROLL vectors a thread takes at a time.
+template <typename T, int G> __host__ __device__ constexpr int mark_words(int n) {
+    return ((n + Vec<T>::N - 1) / Vec<T>::N + UNROLL * G - 1) / (UNROLL * G) * G;
+}
+template <typename T, int G> __device__ __forceinline__ void mark_listed(const int* idx, int k, int first, int n, unsigned* bits, int tid) {
+    constexpr int N = Vec<T>::N;
+    for (int i = tid; i < mark_words<T, G>(n); i += G) bits[i] = 0;
     group_sync<G>();
     for (int i = tid; i < k; i += G) {
         const int v = idx[i] - first;
-        if (idx[i] >= 0 && v >= 0 && v < n) atomicOr(&bits[v >> 5], 1u << (v & 31));
+        if (idx[i] >= 0 && v >= 0 && v < n) {
+            const int vec = v / N;
+            atomicOr(&bits[vec / (UNROLL * G) * G + vec % G], 1u << (vec / G % UNROLL * 8 + v % N));
+        }
     }
     group_sync<G>();
+}
+template <int N> __device__ __forceinline__ void drop_listed(float (&f)[N], unsigned b) {
+    if (b) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) f[j] = (b >> j) & 1u ? -INFINITY : f[j];
+    }
 }
 // the online sums of the classes of a segment, without the listed ones if TAIL
 template <typename T, int G, bool TAIL>
 __device__ __forceinline__ Online distill_stream(const T* __restrict__ z, int n, int tid, const unsigned* bits, float c) {
     constexpr int N = Vec<T>::N;
     Online on;
-    stream_row<T, G>(z, n, tid, [&](const float(&f0)[N], int at) {
-        float f[N];
+    stream_row<T, G>(
+        z, n, tid,
+        [&](const uint4v(&q)[UNROLL], int i) {
+            const unsigned b = TAIL ? bits[i / UNROLL / G * G + tid] : 0u;
+            float f[UNROLL * N], vm = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < N; ++j) f[j] = f0[j];
-        if (TAIL) {
-            const unsigned b = (bits[at >> 5] >> (at & 31)) & ((1u << N) - 1u);
-            if (b) {
+            for (int u = 0; u < UNROLL; ++u) {
+                float x[N];
+                unpack(q[u], x, (T*)nullptr);
+                if (TAIL) drop_listed(x, (b >> (8 * u)) & 0xFFu);
+                vm = fmaxf(vm, max_of(x));
 #pragma unroll
-                for (int j = 0; j < N; ++j) f[j] = (b >> j) & 1u ? -INFINITY : f[j];
+                for (int j = 0; j < N; ++j) f[u * N + j] = x[j];
             }
-        }
-        on.add<N, false>(f, max_of(f), c);
-    });
+            on.add<UNROLL * N, false>(f, vm, c);
+        },
+        [&](const float(&f0)[N], int vec) {
+            float f[N];
+#pragma unroll
+            for (int j = 0; j < N; ++j) f[j] = f0[j];
+            if (TAIL && vec * N < n) drop_listed(f, (bits[vec / (UNROLL * G) * G + vec % G] >> (vec / G % UNROLL * 8)) & 0xFFu);
+            on.add<N, false>(f, max_of(f), c);
+        });
     return on;
 }
 
-// The row's loss and what its gradient needs, from the sums (m, s) over all classes, or over the classes that are not listed (tail).
-// All threads of the group; idx in LDS.
-template <typename T, int G>
-__device__ __forceinline__ RowDistill distill_finish(const DistillArgs& a, const T* __restrict__ z, int64_t classes, ListPos l, const int* idx,
-                                                     float m, float s, int tid, double* red) {
+// The row's loss and what its gradient needs, from the sums over all classes, or over the classes that are not listed (tail).  One
+// wave; every lane gets the result.  What cancels is combined in float64: 1 - sum p, the terms of a good
+// student, log q_rest = -log(1 + listed sum / rest sum).
+__device__ __forceinline__ RowDistill distill_finish(const DistillArgs& a, ListLds d, float m, float s, int lane) {
+    struct { int i[SLOTS]; float t[SLOTS], z[SLOTS]; } l;
+#pragma unroll
+    for (int e = 0; e < SLOTS; ++e) {
+        const int k = lane + 64 * e;
+        l.i[e] = k < a.k ? d.i[k] : -1;
+        l.t[e] = k < a.k ? d.t[k] : -INFINITY;
+        l.z[e] = k < a.k ? d.z[k] : -INFINITY;
+    }
     RowDistill o;
-    o.skip = false;
     bool bad = false;
     float tmax = -INFINITY, zmax = -INFINITY;
-    for (int k = tid; k < a.k; k += G) {
-        const int i = idx[k];
-        if (i < 0) continue;
-        if (i >= classes) { bad = true; continue; }
-        tmax = fmaxf(tmax, load_float(a.teacher, l.base + k * l.stride, a.teacher_dtype));
-        zmax = fmaxf(zmax, to_f32(z[i]));
+#pragma unroll
+    for (int e = 0; e < SLOTS; ++e) {
+        bad |= l.i[e] == 0x7FFFFFFF;
+        tmax = fmaxf(tmax, l.t[e]);
+        zmax = fmaxf(zmax, l.z[e]);
     }
-    zmax = group_max<G>(zmax, red);
-    double norm = 0.0, mass = 1.0, rest = 0.0, log_q_rest = 0.0, lse, lse_rest = 0.0;
-    double M = m, log_s;                                        // maximum and log sum of all classes
+    bad = __any(bad);
+    const double log_m = log_sum(m, s, a.c);                    // log of the streamed sum relative to m
+    const bool have_rest = !(s == 0.f);                         // NaN counts
+    double norm = 0.0, mass = 1.0, rest = 0.0, log_q_rest = 0.0, lse_rest = 0.0;
+    double M = m, log_s = log_m;                                // maximum and log sum of all classes
     if (!a.tail) {
-        tmax = group_max<G>(tmax, red);
-        double e = 0.0;
-        for (int k = tid; k < a.k; k += G) {
-            const int i = idx[k];
-            if (i >= 0 && i < classes) {
-                const float t = load_float(a.teacher, l.base + k * l.stride, a.teacher_dtype);
-                e += tmax == -INFINITY ? (t != t ? (double)t : 0.0) : exp((double)t - tmax);
-            }
-        }
-        e = group_sum<G>(e, red);
-        norm = e == 0.0 ? -INFINITY : (tmax == -INFINITY ? e : tmax + log(e));
-        mass = e == 0.0 ? 0.0 : 1.0;
-        log_s = log((double)s);
+        tmax = wave_max(tmax);
+        double sum = 0.0;
+#pragma unroll
+        for (int e = 0; e < SLOTS; ++e)
+            if (l.i[e] >= 0) sum += tmax == -INFINITY ? (l.t[e] != l.t[e] ? (double)l.t[e] : 0.0) : exp((double)l.t[e] - tmax);
+        sum = wave_sum(sum);
+        norm = sum == 0.0 ? -INFINITY : (tmax == -INFINITY ? sum : tmax + log(sum));
+        mass = sum == 0.0 ? 0.0 : 1.0;
     } else {
+        zmax = wave_max(zmax);
         double sl = 0.0, P = 0.0;
-        for (int k = tid; k < a.k; k += G) {
-            const int i = idx[k];
-            if (i < 0 || i >= classes) continue;
-            P += exp((double)load_float(a.teacher, l.base + k * l.stride, a.teacher_dtype));
+#pragma unroll
+        for (int e = 0; e < SLOTS; ++e) {
+            if (l.i[e] < 0) continue;
+            P += exp((double)l.t[e]);
             bool again = false;
-            for (int j = 0; j < k; ++j) again |= idx[j] == i;
-            const float zk = to_f32(z[i]);
-            if (!again) sl += zmax == -INFINITY ? (zk != zk ? (double)zk : 0.0) : (double)exp2_hw((zk - zmax) * a.c);
+            for (int j = 0; j < lane + 64 * e; ++j) again |= d.i[j] == l.i[e];
+            if (!again) sl += zmax == -INFINITY ? (l.z[e] != l.z[e] ? (double)l.z[e] : 0.0) : (double)exp2_hw((l.z[e] - zmax) * a.c);
         }
-        sl = group_sum<G>(sl, red);
-        P = group_sum<G>(P, red);
-        const bool have_rest = !(s == 0.f);                      // NaN counts
+        sl = wave_sum(sl);
+        P = wave_sum(P);
         rest = have_rest ? (P < 1.0 ? 1.0 - P : 0.0) : 0.0;
         mass = P + rest;
+        lse_rest = (double)m * a.inv_t + log_m;
         if (!have_rest) { M = zmax; log_s = log(sl); }
-        else if (sl == 0.0) { log_s = log((double)s); lse_rest = (double)m * a.inv_t + log_s; }
-        else {
+        else if (sl != 0.0) {
             M = fmaxf(m, zmax);
-            const double u = ((double)zmax - m) * a.inv_t + log(sl) - log((double)s);      // log of (listed sum / rest sum)
+            const double u = ((double)zmax - m) * a.inv_t + log(sl) - log_m;      // log of (listed sum / rest sum)
             log_q_rest = -(u > 700.0 ? u : log1p(exp(u)));
-            lse_rest = (double)m * a.inv_t + log((double)s);
-            log_s = lse_rest - log_q_rest - M * a.inv_t;
+            log_s = ((double)m - M) * a.inv_t + log_m - log_q_rest;
         }
     }
-    lse = M == -INFINITY ? -INFINITY : M * a.inv_t + log_s;
+    const bool empty = M == -INFINITY;
     double sum = 0.0;
-    for (int k = tid; k < a.k; k += G) {
-        const int i = idx[k];
-        if (i < 0 || i >= classes) continue;
-        const double lp = (double)load_float(a.teacher, l.base + k * l.stride, a.teacher_dtype) - norm;
+#pragma unroll
+    for (int e = 0; e < SLOTS; ++e) {
+        if (l.i[e] < 0) continue;
+        const double lp = (double)l.t[e] - norm;
         const double pk = mass == 0.0 ? 0.0 : exp(lp);
-        const double lq = lse == -INFINITY ? -INFINITY : ((double)to_f32(z[i]) - M) * a.inv_t - log_s;
+        const double lq = empty ? -INFINITY : ((double)l.z[e] - M) * a.inv_t - log_s;
         if (!(pk == 0.0)) sum += pk * (lp - lq);
     }
-    if (bad) sum = NAN;
-    sum = group_sum<G>(sum, red);
+    sum = wave_sum(sum);
     if (rest > 0.0) sum += rest * (log(rest) - log_q_rest);
-    const bool nan_row = s != s;
-    o.loss = nan_row ? NAN : (float)(sum * a.t * a.t);
-    o.lse = nan_row ? NAN : (float)lse;
+    if (bad || s != s) sum = NAN;
+    o.loss = (float)(sum * a.t * a.t);
+    o.lse = s != s ? NAN : (empty ? -INFINITY : (float)(M * a.inv_t + log_s));
     o.mass = (float)mass;
     o.norm = (float)norm;
     if (a.tail) {
-        const bool have_rest = !(s == 0.f);
         o.ref = have_rest ? (float)lse_rest : 0.f;
         o.factor = have_rest ? (float)(mass * exp(log_q_rest) - rest) : 0.f;
     } else {
@@ -699,102 +836,74 @@ __device__ __forceinline__ RowDistill distill_finish(const DistillArgs& a, const
     if (sum != sum) o.factor = NAN;                              // an invalid entry shows in the gradient too
     return o;
 }
+__device__ __forceinline__ void write_distill(const DistillArgs& a, const RowDistill& o, int64_t r, int64_t rows) {
+    const float w = a.weight ? a.weight[r] : 1.f;
+    a.loss[r] = w == 0.f ? 0.f : o.loss * w;
+    if (a.aux) {
+        a.aux[r] = o.ref;
+        a.aux[rows + r] = o.factor;
+        a.aux[2 * rows + r] = o.lse;
+        a.aux[3 * rows + r] = a.tail ? o.mass : o.norm;
+    }
+}
 
 template <typename T, int G, bool TAIL>
 __global__ __launch_bounds__(256) void distill_row_kernel(LogitsView v, int64_t rows, DistillArgs a, int segments, int seg_len, Partial* __restrict__ part) {
     constexpr int GROUPS = 256 / G;
     extern __shared__ int dyn[];
-    __shared__ double red[4];
-    const int g = threadIdx.x / G, tid = threadIdx.x % G;
+    __shared__ Partial waves[4];
+    const int g = threadIdx.x / G, tid = threadIdx.x % G, lane = threadIdx.x & 63;
     const int64_t item = (int64_t)blockIdx.x * GROUPS + g;
     if (item >= rows * segments) return;
     const int64_t r = segments == 1 ? item : item / segments;
     const int seg = segments == 1 ? 0 : (int)(item % segments);
-    const int words = TAIL ? (seg_len + 31) / 32 : 0;
-    int* idx = dyn + g * (a.k + words);
-    unsigned* bits = reinterpret_cast<unsigned*>(idx + a.k);
+    const int words = TAIL ? mark_words<T, G>(seg_len) : 0;
+    const ListLds list = list_lds(dyn + g * (3 * a.k + words), a.k);
+    unsigned* bits = reinterpret_cast<unsigned*>(list.z + a.k);
     const RowPos p = row_pos(v, r);
-    const ListPos l = list_pos(v, p, r, a.k);
     const T* z = static_cast<const T*>(v.p) + row_start(v, p);
     const int first = seg * seg_len;
     const int n = (int)(v.classes - first < seg_len ? v.classes - first : seg_len);
-    list_load<T, G>(a, l, tid, idx);
+    if (tid < 64) list_load(a, list_pos(v, p, r, a.k), z, v.classes, lane, list);
     group_sync<G>();
-    if (TAIL) mark_listed<G>(idx, a.k, first, n, bits, tid);
-    Online on = distill_stream<T, G, TAIL>(z + first, n, tid, bits, a.c);
-    const float m = group_max<G>(on.m, red);
-    on.rescale(m, a.c);
-    const float s = (float)group_sum<G>((double)on.s, red);
+    if (TAIL) mark_listed<T, G>(list.i, a.k, first, n, bits, tid);
+    const Online on = group_join<G>(distill_stream<T, G, TAIL>(z + first, n, tid, bits, a.c), a.c, waves);
     if (segments > 1) {
-        if (tid == 0) part[item] = {m, s, 0.f, 0.f};
+        if (tid == 0) part[item] = {on.m, on.s, 0.f, 0.f};
         return;
     }
-    const RowDistill o = distill_finish<T, G>(a, z, v.classes, l, idx, m, s, tid, red);
-    if (tid == 0) {
-        const float w = a.weight ? a.weight[r] : 1.f;
-        a.loss[r] = w == 0.f ? 0.f : o.loss * w;
-        if (a.aux) {
-            a.aux[r] = o.ref;
-            a.aux[rows + r] = o.factor;
-            a.aux[2 * rows + r] = o.lse;
-            a.aux[3 * rows + r] = a.tail ? o.mass : o.norm;
-        }
-    }
+    if (tid >= 64) return;
+    const RowDistill o = distill_finish(a, list, on.m, on.s, lane);
+    if (lane == 0) write_distill(a, o, r, rows);
 }
 template <typename T>
-__global__ __launch_bounds__(256) void distill_join_kernel(LogitsView v, int64_t rows, DistillArgs a, int segments, const Partial* __restrict__ part) {
+__global__ __launch_bounds__(64) void distill_join_kernel(LogitsView v, int64_t rows, DistillArgs a, int segments, const Partial* __restrict__ part) {
     extern __shared__ int dyn[];
-    __shared__ double red[4];
     const int64_t r = blockIdx.x;
-    const int tid = threadIdx.x;
     const RowPos p = row_pos(v, r);
-    const ListPos l = list_pos(v, p, r, a.k);
-    const T* z = static_cast<const T*>(v.p) + row_start(v, p);
-    list_load<T, 256>(a, l, tid, dyn);
-    Online on;
-    for (int i = tid; i < segments; i += 256) {
-        const Partial q = part[r * segments + i];
-        Online b;
-        b.m = q.m; b.s = q.s;
-        const float mn = fmaxf(on.m, q.m);
-        on.rescale(mn, a.c);
-        b.rescale(mn, a.c);
-        on.s += b.s;
-    }
-    const float m = group_max<256>(on.m, red);
-    on.rescale(m, a.c);
-    const float s = (float)group_sum<256>((double)on.s, red);
-    const RowDistill o = distill_finish<T, 256>(a, z, v.classes, l, dyn, m, s, tid, red);
-    if (tid == 0) {
-        const float w = a.weight ? a.weight[r] : 1.f;
-        a.loss[r] = w == 0.f ? 0.f : o.loss * w;
-        if (a.aux) {
-            a.aux[r] = o.ref;
-            a.aux[rows + r] = o.factor;
-            a.aux[2 * rows + r] = o.lse;
-            a.aux[3 * rows + r] = a.tail ? o.mass : o.norm;
-        }
-    }
+    const ListLds list = list_lds(dyn, a.k);
+    list_load(a, list_pos(v, p, r, a.k), static_cast<const T*>(v.p) + row_start(v, p), v.classes, threadIdx.x, list);
+    wave_sync();
+    const Online on = join_segments(part + r * segments, segments, a.c);
+    const RowDistill o = distill_finish(a, list, on.m, on.s, threadIdx.x);
+    if (threadIdx.x == 0) write_distill(a, o, r, rows);
 }
 
 // the listed classes of [first, first + n): overwrites what the sweep wrote there; the first mention of a class writes for all of them
 template <typename T, int G>
-__device__ __forceinline__ void listed_grad(const DistillArgs& a, const T* __restrict__ z, T* __restrict__ out, int64_t classes, ListPos l, const int* idx,
-                                            int64_t first, int64_t n, float lse, float mass, float norm, float scale, int tid) {
+__device__ __forceinline__ void listed_grad(const DistillArgs& a, T* __restrict__ out, ListLds d, int64_t first, int64_t n, float lse, float mass, float norm,
+                                            float scale, int tid) {
     for (int k = tid; k < a.k; k += G) {
-        const int i = idx[k];
-        if (i < 0 || i >= classes || i < first || i >= first + n) continue;
+        const int i = d.i[k];
+        if (i < first || i >= first + n || i < 0 || i == 0x7FFFFFFF) continue;
         bool again = false;
-        for (int j = 0; j < k; ++j) again |= idx[j] == i;
-        if (again) continue;
         float p = 0.f;
-        for (int j = k; j < a.k; ++j)
-            if (idx[j] == i) {
-                const float t = load_float(a.teacher, l.base + j * l.stride, a.teacher_dtype);
-                p += a.tail ? expf(t) : (norm == -INFINITY ? 0.f : expf(t - norm));
-            }
-        const float q = lse == -INFINITY ? 0.f : exp2_hw(fmaf(to_f32(z[i]), a.c, -lse * LOG2E));
-        out[i] = from_f32<T>(lse == -INFINITY ? 0.f : scale * (mass * q - p));
+        for (int j = 0; j < a.k; ++j) {
+            if (d.i[j] != i) continue;
+            again |= j < k;
+            p += a.tail ? expf(d.t[j]) : (norm == -INFINITY ? 0.f : expf(d.t[j] - norm));
+        }
+        if (!again) out[i] = from_f32<T>(scale * (mass * exp2_hw(fmaf(d.z[k], a.c, -lse * LOG2E)) - p));
     }
 }
 __device__ __forceinline__ float unlisted_grad(float z, float ref2, float f, float c) { return f * exp2_hw(fmaf(z, c, -ref2)); }
@@ -808,77 +917,139 @@ __global__ __launch_bounds__(256) void distill_grad_row_kernel(LogitsView v, int
     if (item >= rows * chunks) return;
     const int64_t r = chunks == 1 ? item : item / chunks;
     const int first = chunks == 1 ? 0 : (int)(item % chunks) * CHUNK;
-    int* idx = dyn + g * a.k;
+    const ListLds list = list_lds(dyn + g * 3 * a.k, a.k);
     const RowPos p = row_pos(v, r);
-    const ListPos l = list_pos(v, p, r, a.k);
-    list_load<T, G>(a, l, tid, idx);
     const T* z = static_cast<const T*>(v.p) + row_start(v, p);
+    if (tid < 64) list_load(a, list_pos(v, p, r, a.k), z, v.classes, tid, list);
     T* out = grad + r * v.classes;
-    const float up = (a.g_loss ? a.g_loss[r] : 1.f) * (a.weight ? a.weight[r] : 1.f);
-    const float scale = up * a.t;
+    const float w = a.weight ? a.weight[r] : 1.f;
+    const float scale = (a.g_loss ? a.g_loss[r] : 1.f) * w * a.t;
     const float ref = a.aux[r], factor = a.aux[rows + r], lse = a.aux[2 * rows + r], x = a.aux[3 * rows + r];
     const float mass = a.tail ? x : (x == -INFINITY ? 0.f : 1.f), norm = a.tail ? 0.f : x;
-    const bool none = lse == -INFINITY || (a.weight && a.weight[r] == 0.f);
+    const bool none = lse == -INFINITY || w == 0.f;
     const float ref2 = none ? 0.f : ref * LOG2E, f = scale * factor;
     map_chunk<T, G>(z, out, first, v.classes, tid, [&](float y, int64_t) { return none ? 0.f : unlisted_grad(y, ref2, f, a.c); });
     group_sync<G>();
-    if (!none) listed_grad<T, G>(a, z, out, v.classes, l, idx, first, CHUNK, lse, mass, norm, scale, tid);
+    if (!none) listed_grad<T, G>(a, out, list, first, CHUNK, lse, mass, norm, scale, tid);
 }
 
-// loss and gradient in one kernel: the row is read twice, the second time from cache, and its gradient written
+// Loss and gradient in one kernel, the row in the registers of G threads (HELD vectors each) between its one read and its gradient's
+// write.  A second read of a row of 256 KB would come from HBM: the rows in flight are larger than the caches.
+constexpr int HELD = 16;
+// the compiler may not carry what it unpacked from q past this point (two or four times the registers of q itself)
+__device__ __forceinline__ void keep_packed(uint4v (&q)[HELD]) {
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) asm volatile("" : "+v"(q[h]));
+}
 template <typename T, int G, bool TAIL>
-__global__ __launch_bounds__(256) void distill_step_row_kernel(LogitsView v, int64_t rows, DistillArgs a, T* __restrict__ grad) {
-    constexpr int GROUPS = 256 / G, N = Vec<T>::N;
+__global__ __launch_bounds__(G < 256 ? 256 : G, 4) void distill_step_kernel(LogitsView v, int64_t rows, DistillArgs a, T* __restrict__ grad) {
+    constexpr int BLOCK = G < 256 ? 256 : G, GROUPS = BLOCK / G, N = Vec<T>::N;
     extern __shared__ int dyn[];
-    __shared__ double red[4];
-    const int g = threadIdx.x / G, tid = threadIdx.x % G;
+    __shared__ Partial waves[BLOCK / 64];
+    __shared__ RowDistill shared_row;
+    const int g = threadIdx.x / G, tid = threadIdx.x % G, lane = threadIdx.x & 63;
     const int64_t r = (int64_t)blockIdx.x * GROUPS + g;
     if (r >= rows) return;
-    const int words = TAIL ? (int)((v.classes + 31) / 32) : 0;
-    int* idx = dyn + g * (a.k + words);
-    unsigned* bits = reinterpret_cast<unsigned*>(idx + a.k);
+    const int n = (int)v.classes, nfull = n / N;
+    const int words = TAIL ? mark_words<T, G>(n) : 0;
+    const ListLds list = list_lds(dyn + g * (3 * a.k + words), a.k);
+    unsigned* bits = reinterpret_cast<unsigned*>(list.z + a.k);
     const RowPos p = row_pos(v, r);
-    const ListPos l = list_pos(v, p, r, a.k);
     const T* z = static_cast<const T*>(v.p) + row_start(v, p);
     T* out = grad + r * v.classes;
     const float w = a.weight ? a.weight[r] : 1.f;
-    list_load<T, G>(a, l, tid, idx);
+    uint4v q[HELD];                                             // beyond the row: -inf
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+        q[h] = raw_neg_inf<T>();
+        if (tid + h * G < nfull) q[h] = load_raw(z + (int64_t)(tid + h * G) * N);
+    }
+    const bool has_edge = nfull * N < n && nfull % G == tid;    // the last, partial vector
+    float edge[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) edge[j] = has_edge && nfull * N + j < n ? to_f32(z[nfull * N + j]) : -INFINITY;
+    if (tid < 64) list_load(a, list_pos(v, p, r, a.k), z, v.classes, lane, list);
     group_sync<G>();
-    if (TAIL) mark_listed<G>(idx, a.k, 0, (int)v.classes, bits, tid);
-    Online on = distill_stream<T, G, TAIL>(z, (int)v.classes, tid, bits, a.c);
-    const float m = group_max<G>(on.m, red);
-    on.rescale(m, a.c);
-    const float s = (float)group_sum<G>((double)on.s, red);
-    const RowDistill o = distill_finish<T, G>(a, z, v.classes, l, idx, m, s, tid, red);
-    if (tid == 0) a.loss[r] = w == 0.f ? 0.f : o.loss * w;
+    if (TAIL) mark_listed<T, G>(list.i, a.k, 0, n, bits, tid);
+    // (tail) the listed classes leave the registers: their logits and gradients come from the list
+    Online on;
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+        if (h * G >= nfull) continue;                           // of the whole group
+        if (TAIL) {
+            const unsigned b = (bits[h / UNROLL * G + tid] >> (h % UNROLL * 8)) & 0xFFu;
+            if (b) q[h] = raw_drop(q[h], b, (T*)nullptr);
+        }
+        float x[N];
+        unpack(q[h], x, (T*)nullptr);
+        on.m = fmaxf(on.m, max_of(x));
+    }
+    if (has_edge) {
+        if (TAIL) drop_listed(edge, (bits[nfull / (UNROLL * G) * G + tid] >> (nfull / G % UNROLL * 8)) & 0xFFu);
+        on.m = fmaxf(on.m, max_of(edge));
+    }
+    keep_packed(q);
+    const auto sums = [&](auto far_) {
+        constexpr bool FAR = decltype(far_)::value;             // some lane's maximum is -inf, or beyond BIG
+        const bool far = FAR && !(fabsf(on.m) <= BIG);
+        const float R = far ? 0.f : reference(on.m, a.c), sub = on.m == -INFINITY ? 0.f : on.m;
+        const auto term = [&](float f) { return exp2_hw(FAR && far ? (f - sub) * a.c : fmaf(f, a.c, -R)); };
+#pragma unroll
+        for (int h = 0; h < HELD; ++h) {
+            if (h * G >= nfull) continue;
+            float x[N];
+            unpack(q[h], x, (T*)nullptr);
+#pragma unroll
+            for (int j = 0; j < N; ++j) on.s += term(x[j]);
+        }
+        if (has_edge) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) on.s += term(edge[j]);
+        }
+    };
+    if (__builtin_expect(__any(!(fabsf(on.m) <= BIG)), 0)) sums(std::true_type());
+    else sums(std::false_type());
+    keep_packed(q);
+    on = group_join<G>(on, a.c, waves);
+    RowDistill o;
+    if (tid < 64) {
+        o = distill_finish(a, list, on.m, on.s, lane);
+        if (lane == 0) a.loss[r] = w == 0.f ? 0.f : o.loss * w;
+    }
+    if (G > 64) {
+        if (threadIdx.x == 0) shared_row = o;
+        __syncthreads();
+        o = shared_row;
+    }
     const float scale = w * a.t;
     const bool none = o.lse == -INFINITY || w == 0.f;
     const float ref2 = none ? 0.f : o.ref * LOG2E, f = scale * o.factor;
-    stream_row<T, G>(z, (int)v.classes, tid, [&](const float(&y)[N], int at) {
-        float d[N];
 #pragma unroll
-        for (int j = 0; j < N; ++j) d[j] = none ? 0.f : unlisted_grad(y[j], ref2, f, a.c);
-        if (at + N <= v.classes) store_vec(out + at, d);
-        else {
-            for (int j = 0; j < N; ++j)
-                if (at + j < v.classes) out[at + j] = from_f32<T>(d[j]);
+    for (int h = 0; h < HELD; ++h) {
+        if (tid + h * G < nfull) {
+            float x[N];
+            unpack(q[h], x, (T*)nullptr);
+#pragma unroll
+            for (int j = 0; j < N; ++j) x[j] = none ? 0.f : unlisted_grad(x[j], ref2, f, a.c);
+            store_vec(out + (int64_t)(tid + h * G) * N, x);
         }
-    });
+    }
+    if (has_edge) {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (nfull * N + j < n) out[nfull * N + j] = from_f32<T>(none ? 0.f : unlisted_grad(edge[j], ref2, f, a.c));
+    }
     group_sync<G>();
-    if (!none) listed_grad<T, G>(a, z, out, v.classes, l, idx, 0, v.classes, o.lse, o.mass, o.norm, scale, tid);
+    if (!none) listed_grad<T, G>(a, out, list, 0, n, o.lse, o.mass, o.norm, scale, tid);
 }
 
 // ========================================================================================================================================
 // rows of few classes, at any stride: a thread per row, the classes in registers
 // ========================================================================================================================================
-template <int CM> struct ColRow {
-    float z[CM];
-    float m, s;
-    template <typename T> __device__ __forceinline__ void load(const T* p, int64_t sc, int classes) {
+template <int CM, typename T> __device__ __forceinline__ void load_classes(float (&z)[CM], const T* p, int64_t sc, int classes) {
 #pragma unroll
-        for (int c = 0; c < CM; ++c) z[c] = c < classes ? to_f32(p[c * sc]) : -INFINITY;
-    }
-};
+    for (int c = 0; c < CM; ++c) z[c] = c < classes ? to_f32(p[c * sc]) : -INFINITY;
+}
 
 template <typename T, int CM>
 __global__ __launch_bounds__(256) void score_col_kernel(LogitsView v, int64_t rows, ScoreOut o) {
@@ -886,26 +1057,36 @@ __global__ __launch_bounds__(256) void score_col_kernel(LogitsView v, int64_t ro
     if (r >= rows) return;
     const int classes = (int)v.classes;
     const RowPos p = row_pos(v, r);
-    const T* z = static_cast<const T*>(v.p) + row_start(v, p);
-    ColRow<CM> x;
-    x.load(z, v.sc, classes);
-    Online on;
-    on.add<CM, true>(x.z, max_of(x.z), o.c);
-    write_row<T>(o, z, v.sc, classes, r, on.m, on.s, on.w);
-    if (o.top) {
-        const float log_s = (float)log((double)on.s);
-        const ListPos l = list_pos(v, p, r, o.top);
-        u64 last = ~0ull;
-        for (int k = 0; k < o.top; ++k) {                      // the largest key below the last one
-            u64 best = 0;
+    const T* zp = static_cast<const T*>(v.p) + row_start(v, p);
+    float z[CM];
+    load_classes(z, zp, v.sc, classes);
+    Online on;                                                  // sums relative to the maximum itself: a row of one class scores exactly 0
+    on.m = max_of(z);
+    const float ref = on.m == -INFINITY ? 0.f : on.m;
 #pragma unroll
-            for (int c = 0; c < CM; ++c) {
-                const u64 key = make_key(order_key(x.z[c]), c);
-                if (c < classes && key < last && key > best) best = key;
-            }
-            last = best;
-            o.top_logprob[l.base + k * l.stride] = on.s != on.s ? on.s : class_logprob(key_value((unsigned)(best >> 32)), on.m, log_s, o.inv_t);
-            o.top_index[l.base + k * l.stride] = (int)key_index(best);
+    for (int c = 0; c < CM; ++c) {
+        const float x = (z[c] - ref) * o.c, e = exp2_hw(x);
+        on.s += e;
+        on.w = fmaf(e, fmaxf(x, NEG_BIG), on.w);
+    }
+    const float log_s = logf(on.s);
+    write_row<T, float>(o, zp, v.sc, classes, r, on.m, on.s, on.w, log_s);
+    if (o.top) {
+        const ListPos l = list_pos(v, p, r, o.top);
+        unsigned key[CM];
+#pragma unroll
+        for (int c = 0; c < CM; ++c) key[c] = c < classes ? order_key(z[c]) : 0u;      // 0: taken
+        for (int k = 0; k < o.top; ++k) {
+            unsigned best = 0;
+#pragma unroll
+            for (int c = 0; c < CM; ++c) best = max(best, key[c]);
+            int at = 0;
+#pragma unroll
+            for (int c = CM - 1; c >= 0; --c) at = key[c] == best ? c : at;             // the lowest
+#pragma unroll
+            for (int c = 0; c < CM; ++c) key[c] = c == at ? 0u : key[c];
+            o.top_logprob[l.base + k * l.stride] = on.s != on.s ? on.s : class_logprob<float>(key_value(best), on.m, log_s, o.inv_t);
+            o.top_index[l.base + k * l.stride] = at;
         }
     }
 }
@@ -918,17 +1099,19 @@ __global__ __launch_bounds__(256) void score_grad_col_kernel(LogitsView v, int64
     if (r >= rows) return;
     const int classes = (int)v.classes;
     const RowPos p = row_pos(v, r);
-    ColRow<CM> x;
-    x.load(static_cast<const T*>(v.p) + row_start(v, p), v.sc, classes);
+    float z[CM];
+    load_classes(z, static_cast<const T*>(v.p) + row_start(v, p), v.sc, classes);
     const RowGrad g = row_grad(o, classes, r);
     T* out = grad + grad_start(v, p, r);
     const int64_t step = v.class_last ? 1 : v.inner;
 #pragma unroll
     for (int c = 0; c < CM; ++c)
-        if (c < classes) out[c * step] = from_f32<T>(grad_value(g, x.z[c], o.c) + (c == g.token ? g.at_token : 0.f));
+        if (c < classes) out[c * step] = from_f32<T>(grad_value(g, z[c], o.c) + (c == g.token ? g.at_token : 0.f));
 }
 
-// loss (a.loss) and / or gradient (grad) of a row; the gradient's scale: weight or the upstream gradient
+// Loss (a.loss) and / or gradient (grad) of a row; the gradient's scale: weight or the upstream gradient.  In float32 but for 1 - sum p,
+// which cancels: a few classes leave sums of a few roundings.  The exponentials relative to the row's maximum are kept for the gradient
+// (recomputed relative to the rest's maximum where the rest would underflow).
 template <typename T, int CM, bool LOSS, bool GRAD>
 __global__ __launch_bounds__(256) void distill_col_kernel(LogitsView v, int64_t rows, DistillArgs a, T* __restrict__ grad) {
     const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -936,100 +1119,94 @@ __global__ __launch_bounds__(256) void distill_col_kernel(LogitsView v, int64_t 
     const int classes = (int)v.classes;
     const RowPos p = row_pos(v, r);
     const ListPos l = list_pos(v, p, r, a.k);
-    const T* z = static_cast<const T*>(v.p) + row_start(v, p);
-    ColRow<CM> x;
-    x.load(z, v.sc, classes);
+    float z[CM], e[CM], target[CM];
+    load_classes(z, static_cast<const T*>(v.p) + row_start(v, p), v.sc, classes);
     const float w = a.weight ? a.weight[r] : 1.f;
-    // the teacher's probability of each class
-    float target[CM];
+    // the teacher: tail: p = e^t, r = 1 - sum p;  else p = e^{t - norm}
+    double total = 0.0;
+    float norm = 0.f;
+    if (a.tail) {
+        for (int k = 0; k < a.k; ++k)
+            if (load_int(a.index, l.base + k * l.stride, a.index_bytes) >= 0) total += exp((double)load_float(a.teacher, l.base + k * l.stride, a.teacher_dtype));
+    } else {
+        float tmax = -INFINITY, sum = 0.f;
+        for (int k = 0; k < a.k; ++k)
+            if (load_int(a.index, l.base + k * l.stride, a.index_bytes) >= 0) tmax = fmaxf(tmax, load_float(a.teacher, l.base + k * l.stride, a.teacher_dtype));
+        for (int k = 0; k < a.k; ++k) {
+            if (load_int(a.index, l.base + k * l.stride, a.index_bytes) < 0) continue;
+            const float t = load_float(a.teacher, l.base + k * l.stride, a.teacher_dtype);
+            sum += tmax == -INFINITY ? (t != t ? t : 0.f) : exp2_hw((t - tmax) * LOG2E);
+        }
+        norm = sum == 0.f ? -INFINITY : (tmax == -INFINITY ? sum : tmax + logf(sum));
+    }
+    const bool nobody = !a.tail && norm == -INFINITY;                       // no entry has any probability
+    const float m = max_of(z), ref = m == -INFINITY ? 0.f : m;
+    float s = 0.f;
 #pragma unroll
-    for (int c = 0; c < CM; ++c) target[c] = 0.f;
+    for (int c = 0; c < CM; ++c) {
+        e[c] = exp2_hw((z[c] - ref) * a.c);
+        s += e[c];
+        target[c] = 0.f;
+    }
+    const bool empty = m == -INFINITY;
+    const float log_s = logf(s);
     u64 listed = 0;
     bool bad = false;
-    float tmax = -INFINITY;
-    double norm = 0.0, P = 0.0;
-    if (!a.tail) {
-        for (int k = 0; k < a.k; ++k) {
-            const int64_t i = load_int(a.index, l.base + k * l.stride, a.index_bytes);
-            if (i >= 0) tmax = fmaxf(tmax, load_float(a.teacher, l.base + k * l.stride, a.teacher_dtype));
-        }
-        double e = 0.0;
-        for (int k = 0; k < a.k; ++k) {
-            const int64_t i = load_int(a.index, l.base + k * l.stride, a.index_bytes);
-            const float t = load_float(a.teacher, l.base + k * l.stride, a.teacher_dtype);
-            if (i >= 0) e += tmax == -INFINITY ? (t != t ? (double)t : 0.0) : exp((double)t - tmax);
-        }
-        norm = e == 0.0 ? -INFINITY : (tmax == -INFINITY ? e : tmax + log(e));
-    }
-    const float m_all = max_of(x.z);
-    Online on;
-    on.add<CM, false>(x.z, m_all, a.c);
-    const bool empty = on.s == 0.f;
-    const double log_all = log((double)on.s);
-    double sum = 0.0;
+    float sum = 0.f;
     for (int k = 0; k < a.k; ++k) {
         const int64_t i = load_int(a.index, l.base + k * l.stride, a.index_bytes);
         if (i < 0) continue;
         if (i >= classes) { bad = true; continue; }
-        const double lp = (double)load_float(a.teacher, l.base + k * l.stride, a.teacher_dtype) - norm;
-        const double pk = norm == -INFINITY ? 0.0 : exp(lp);
-        P += pk;
+        const float lp = load_float(a.teacher, l.base + k * l.stride, a.teacher_dtype) - norm;
+        const float pk = nobody ? 0.f : exp2_hw(lp * LOG2E);
         listed |= 1ull << i;
         float zk = 0.f;
 #pragma unroll
         for (int c = 0; c < CM; ++c) {
-            if (c == (int)i) { zk = x.z[c]; target[c] += (float)pk; }
+            zk = c == (int)i ? z[c] : zk;
+            target[c] += c == (int)i ? pk : 0.f;
         }
-        if (LOSS && !(pk == 0.0)) sum += pk * (lp - (empty ? -INFINITY : ((double)zk - m_all) * a.inv_t - log_all));
+        if (LOSS && !(pk == 0.f)) sum += pk * (lp - (empty ? -INFINITY : fmaf(zk - m, a.inv_t, -log_s)));
     }
-    double mass = a.tail ? P : (norm == -INFINITY ? 0.0 : 1.0), rest = 0.0, q_rest = 1.0;
-    float m_rest = m_all, s_rest = on.s;
+    float mass = nobody ? 0.f : 1.f, rest = 0.f, log_q_rest = 0.f, s_rest = 0.f;
     if (a.tail) {
-        m_rest = -INFINITY;
-#pragma unroll
-        for (int c = 0; c < CM; ++c)
-            if (!((listed >> c) & 1)) m_rest = fmaxf(m_rest, x.z[c]);
-        const float refm = m_rest == -INFINITY ? 0.f : m_rest;
-        s_rest = 0.f;
-        float s_list = 0.f;
-        const float ref_all = m_all == -INFINITY ? 0.f : m_all;
+        float m_rest = -INFINITY;
 #pragma unroll
         for (int c = 0; c < CM; ++c) {
             const bool in = (listed >> c) & 1;
-            const float e = exp2_hw((x.z[c] - (in ? ref_all : refm)) * a.c);
-            s_rest += in ? 0.f : e;
-            s_list += in ? e : 0.f;
+            m_rest = fmaxf(m_rest, in ? -INFINITY : z[c]);
+            s_rest += in ? 0.f : e[c];
         }
-        if (s_rest > 0.f) {
-            rest = P < 1.0 ? 1.0 - P : 0.0;
-            mass = P + rest;
-            double lq = 0.0;
-            if (s_list > 0.f) {
-                const double u = ((double)m_all - m_rest) * a.inv_t + log((double)s_list / s_rest);
-                lq = -(u > 700.0 ? u : log1p(exp(u)));
+        float shift = 0.f;
+        if (m_rest > -INFINITY && (m_rest - m) * a.c < -60.f) {             // far below the listed ones: relative to its own maximum
+            shift = (m_rest - m) * a.inv_t;
+            s_rest = 0.f;
+#pragma unroll
+            for (int c = 0; c < CM; ++c) {
+                if (!((listed >> c) & 1)) {
+                    e[c] = exp2_hw((z[c] - m_rest) * a.c);
+                    s_rest += e[c];
+                }
             }
-            q_rest = exp(lq);
-            if (LOSS && rest > 0.0) sum += rest * (log(rest) - lq);
         }
+        rest = s_rest > 0.f && total < 1.0 ? (float)(1.0 - total) : 0.f;
+        if (!(rest > 0.f)) mass = (float)total;
+        log_q_rest = shift + logf(s_rest) - log_s;
+        if (LOSS && rest > 0.f) sum += rest * (logf(rest) - log_q_rest);
     }
-    if (bad) sum = NAN;
-    if (LOSS) a.loss[r] = w == 0.f ? 0.f : (float)((on.s != on.s ? NAN : sum * a.t * a.t)) * w;
+    const bool nan = bad || s != s || sum != sum;
+    if (LOSS) a.loss[r] = w == 0.f ? 0.f : (nan ? NAN : sum * a.t * a.t) * w;
     if (GRAD) {
-        const float up = (a.g_loss ? a.g_loss[r] : 1.f) * w;
-        const float scale = up * a.t;
-        const bool none = empty || (a.weight && w == 0.f);
-        const float inv_all = 1.0f / on.s, inv_rest = s_rest > 0.f ? (float)((mass * q_rest - rest) / s_rest) : 0.f;
-        const float ref_all = m_all == -INFINITY ? 0.f : m_all, ref_rest = m_rest == -INFINITY ? 0.f : m_rest;
-        const float fm = (float)mass;
+        const float scale = (a.g_loss ? a.g_loss[r] : 1.f) * w * a.t;
+        const bool none = empty || w == 0.f;
+        const float in_f = scale * mass / s, out_f = a.tail ? (s_rest > 0.f ? scale * (mass * expf(log_q_rest) - rest) / s_rest : 0.f) : in_f;
         T* out = grad + grad_start(v, p, r);
         const int64_t step = v.class_last ? 1 : v.inner;
 #pragma unroll
         for (int c = 0; c < CM; ++c) {
             if (c < classes) {
-                const bool in = !a.tail || ((listed >> c) & 1);
-                const float e = exp2_hw((x.z[c] - (in ? ref_all : ref_rest)) * a.c);
-                const float d = in ? fmaf(fm * inv_all, e, -target[c]) : inv_rest * e;
-                out[c * step] = from_f32<T>(none ? 0.f : (bad || on.s != on.s ? NAN : scale * d));
+                const float d = (listed >> c) & 1 ? fmaf(in_f, e[c], -scale * target[c]) : out_f * e[c];
+                out[c * step] = from_f32<T>(none ? 0.f : (nan ? NAN : d));
             }
         }
     }
@@ -1040,42 +1217,46 @@ __global__ __launch_bounds__(256) void distill_col_kernel(LogitsView v, int64_t 
 // ---- launchers ---------------------------------------------------------------------------------------------------------------------------
 namespace {
 int vec_elems(int dtype) { return dtype == MICA_F32 ? 4 : 8; }
-}  // namespace
+// rows of up to 4096 classes take a wave each, longer ones a block
+bool wave_rows(const LogitsView& v) { return v.classes <= 4096; }
+unsigned blocks_of(int64_t items, int per) { return (unsigned)((items + per - 1) / per); }
 
-bool score_is_col(const LogitsView& v) { return v.classes <= SCORE_COL_MAX; }
-
-// Rows of up to WAVE_MAX classes take a wave each, longer ones a block.
-static bool wave_rows(const LogitsView& v) { return v.classes <= 4096; }
-
-// Few long rows: cut so that about 512 blocks have work, no segment below 8192 classes
-SegPlan score_segments(const LogitsView& v, int64_t rows) {
-    SegPlan s;
-    s.n = 1;
-    s.len = (int)v.classes;
-    if (wave_rows(v)) return s;
-    int64_t n = rows >= 512 ? 1 : 512 / rows;
-    n = std::min<int64_t>(n, (v.classes + 4095) / 4096);
-    n = std::max<int64_t>(n, (v.classes + SCORE_SEG_MAX - 1) / SCORE_SEG_MAX);
-    if (n <= 1) return s;
-    int64_t len = (v.classes + n - 1) / n;
-    len = (len + 511) / 512 * 512;                          // 16-byte vectors of a segment begin where the row's do; bitmap words too
-    s.len = (int)len;
-    s.n = (int)((v.classes + len - 1) / len);
-    return s;
-}
-
-template <typename F> static void by_dtype(int dtype, F&& f) {
+template <typename F> void by_dtype(int dtype, F&& f) {
     if (dtype == MICA_F32) f((float*)nullptr);
     else if (dtype == MICA_BF16) f((bf16_t*)nullptr);
     else f((f16_t*)nullptr);
 }
-template <typename F> static void by_classes(int64_t c, F&& f) {
+template <typename F> void by_classes(int64_t c, F&& f) {
     if (c <= 8) f(std::integral_constant<int, 8>());
     else if (c <= 24) f(std::integral_constant<int, 24>());
     else if (c <= 32) f(std::integral_constant<int, 32>());
     else f(std::integral_constant<int, 64>());
 }
-static unsigned blocks_of(int64_t items, int per) { return (unsigned)((items + per - 1) / per); }
+template <typename F> void by_bool(bool b, F&& f) {
+    if (b) f(std::true_type());
+    else f(std::false_type());
+}
+}  // namespace
+
+bool score_is_col(const LogitsView& v) { return v.classes <= SCORE_COL_MAX; }
+
+// Few long rows: cut so that about 512 blocks have work, no segment below 4096 classes; and no segment beyond what a block's bits take
+SegPlan score_segments(const LogitsView& v, int64_t rows) {
+    SegPlan s;
+    s.n = 1;
+    s.len = (int)v.classes;
+    if (wave_rows(v)) return s;
+    const int64_t longest = SCORE_SEG_BYTES / 16 * vec_elems(v.dtype);
+    int64_t n = rows >= 512 ? 1 : 512 / rows;
+    n = std::min<int64_t>(n, (v.classes + 4095) / 4096);
+    n = std::max<int64_t>(n, (v.classes + longest - 1) / longest);
+    if (n <= 1) return s;
+    int64_t len = (v.classes + n - 1) / n;
+    len = (len + 511) / 512 * 512;                          // 16-byte vectors of a segment begin where the row's do
+    s.len = (int)len;
+    s.n = (int)((v.classes + len - 1) / len);
+    return s;
+}
 
 int64_t score_ws_bytes(const LogitsView& v, int64_t rows, int top) {
     if (score_is_col(v)) return 0;
@@ -1098,17 +1279,12 @@ void launch_score(const LogitsView& v, int64_t rows, const void* tokens, int tok
         Partial* part = static_cast<Partial*>(ws);
         u64* part_top = reinterpret_cast<u64*>(part + rows * s.n);
         const int64_t items = rows * s.n;
-        if (wave_rows(v)) {
-            if (top) hipLaunchKernelGGL((score_row_kernel<T, 64, true>), dim3(blocks_of(items, 4)), dim3(256), 0, st, v, rows, o, s.n, s.len, part, part_top);
-            else hipLaunchKernelGGL((score_row_kernel<T, 64, false>), dim3(blocks_of(items, 4)), dim3(256), 0, st, v, rows, o, s.n, s.len, part, part_top);
-        } else {
-            if (top) hipLaunchKernelGGL((score_row_kernel<T, 256, true>), dim3((unsigned)items), dim3(256), 0, st, v, rows, o, s.n, s.len, part, part_top);
-            else hipLaunchKernelGGL((score_row_kernel<T, 256, false>), dim3((unsigned)items), dim3(256), 0, st, v, rows, o, s.n, s.len, part, part_top);
-        }
-        if (s.n > 1) {
-            if (top) hipLaunchKernelGGL((score_join_kernel<T, true>), dim3((unsigned)rows), dim3(256), 0, st, v, o, s.n, part, part_top);
-            else hipLaunchKernelGGL((score_join_kernel<T, false>), dim3((unsigned)rows), dim3(256), 0, st, v, o, s.n, part, part_top);
-        }
+        by_bool(top > 0, [&](auto has_top) {
+            constexpr bool TOP = decltype(has_top)::value;
+            if (wave_rows(v)) hipLaunchKernelGGL((score_row_kernel<T, 64, TOP>), dim3(blocks_of(items, 4)), dim3(256), 0, st, v, rows, o, s.n, s.len, part, part_top);
+            else hipLaunchKernelGGL((score_row_kernel<T, 256, TOP>), dim3((unsigned)items), dim3(256), 0, st, v, rows, o, s.n, s.len, part, part_top);
+            if (s.n > 1) hipLaunchKernelGGL((score_join_kernel<T, TOP>), dim3((unsigned)rows), dim3(TOP ? JOIN : 64), 0, st, v, o, s.n, part, part_top);
+        });
     });
 }
 
@@ -1131,11 +1307,19 @@ void launch_score_grad(const LogitsView& v, int64_t rows, const void* tokens, in
     });
 }
 
+// threads that hold a row in distill_step_kernel; 0: the row is too long, or rows are too few for a block each
+static int step_group(const LogitsView& v, int64_t rows) {
+    if (score_segments(v, rows).n > 1) return 0;
+    const int64_t nvec = v.classes / vec_elems(v.dtype);
+    for (int g : {64, 256, 512, 1024})
+        if (nvec <= (int64_t)HELD * g) return g;
+    return 0;
+}
+
 int64_t distill_ws_bytes(const LogitsView& v, int64_t rows, bool step) {
     if (score_is_col(v)) return 0;
     const SegPlan s = score_segments(v, rows);
-    if (s.n == 1) return 0;
-    return rows * s.n * (int64_t)sizeof(Partial) + (step ? rows * 16 : 0);
+    return (s.n > 1 ? rows * s.n * (int64_t)sizeof(Partial) : 0) + (step && !step_group(v, rows) ? rows * 16 : 0);
 }
 
 static void distill_loss_rows(const LogitsView& v, int64_t rows, const DistillArgs& a, void* ws, hipStream_t st) {
@@ -1144,15 +1328,16 @@ static void distill_loss_rows(const LogitsView& v, int64_t rows, const DistillAr
         const SegPlan s = score_segments(v, rows);
         Partial* part = static_cast<Partial*>(ws);
         const int64_t items = rows * s.n;
-        const unsigned per = 4u * (a.k + (a.tail ? (s.len + 31) / 32 : 0));
-        if (wave_rows(v)) {
-            if (a.tail) hipLaunchKernelGGL((distill_row_kernel<T, 64, true>), dim3(blocks_of(items, 4)), dim3(256), per * 4, st, v, rows, a, s.n, s.len, part);
-            else hipLaunchKernelGGL((distill_row_kernel<T, 64, false>), dim3(blocks_of(items, 4)), dim3(256), per * 4, st, v, rows, a, s.n, s.len, part);
-        } else {
-            if (a.tail) hipLaunchKernelGGL((distill_row_kernel<T, 256, true>), dim3((unsigned)items), dim3(256), per, st, v, rows, a, s.n, s.len, part);
-            else hipLaunchKernelGGL((distill_row_kernel<T, 256, false>), dim3((unsigned)items), dim3(256), per, st, v, rows, a, s.n, s.len, part);
-        }
-        if (s.n > 1) hipLaunchKernelGGL((distill_join_kernel<T>), dim3((unsigned)rows), dim3(256), 4u * a.k, st, v, rows, a, s.n, part);
+        by_bool(a.tail, [&](auto tail) {
+            constexpr bool TAIL = decltype(tail)::value;
+            if (wave_rows(v))
+                hipLaunchKernelGGL((distill_row_kernel<T, 64, TAIL>), dim3(blocks_of(items, 4)), dim3(256), 16u * (3 * a.k + (TAIL ? mark_words<T, 64>(s.len) : 0)), st, v,
+                                   rows, a, s.n, s.len, part);
+            else
+                hipLaunchKernelGGL((distill_row_kernel<T, 256, TAIL>), dim3((unsigned)items), dim3(256), 4u * (3 * a.k + (TAIL ? mark_words<T, 256>(s.len) : 0)), st, v,
+                                   rows, a, s.n, s.len, part);
+        });
+        if (s.n > 1) hipLaunchKernelGGL((distill_join_kernel<T>), dim3((unsigned)rows), dim3(64), LIST_BYTES * a.k, st, v, rows, a, s.n, part);
     });
 }
 static void distill_grad_rows(const LogitsView& v, int64_t rows, const DistillArgs& a, void* grad, hipStream_t st) {
@@ -1161,8 +1346,8 @@ static void distill_grad_rows(const LogitsView& v, int64_t rows, const DistillAr
         T* out = static_cast<T*>(grad);
         const int g = wave_rows(v) ? 64 : 256, chunk = g * UNROLL * vec_elems(v.dtype);
         const int chunks = (int)((v.classes + chunk - 1) / chunk);
-        if (g == 64) hipLaunchKernelGGL((distill_grad_row_kernel<T, 64>), dim3(blocks_of(rows * chunks, 4)), dim3(256), 16u * a.k, st, v, rows, a, chunks, out);
-        else hipLaunchKernelGGL((distill_grad_row_kernel<T, 256>), dim3((unsigned)(rows * chunks)), dim3(256), 4u * a.k, st, v, rows, a, chunks, out);
+        if (g == 64) hipLaunchKernelGGL((distill_grad_row_kernel<T, 64>), dim3(blocks_of(rows * chunks, 4)), dim3(256), 4 * LIST_BYTES * a.k, st, v, rows, a, chunks, out);
+        else hipLaunchKernelGGL((distill_grad_row_kernel<T, 256>), dim3((unsigned)(rows * chunks)), dim3(256), LIST_BYTES * a.k, st, v, rows, a, chunks, out);
     });
 }
 template <bool LOSS, bool GRAD> static void distill_col(const LogitsView& v, int64_t rows, const DistillArgs& a, void* grad, hipStream_t st) {
@@ -1209,9 +1394,10 @@ void launch_distill_step(const LogitsView& v, int64_t rows, const DistillList& d
     a.weight = weight;
     a.loss = loss;
     if (score_is_col(v)) { distill_col<true, true>(v, rows, a, grad, st); return; }
-    const SegPlan s = score_segments(v, rows);
-    if (s.n > 1) {                                          // few long rows: the segments' sums first
-        a.aux = reinterpret_cast<float*>(static_cast<Partial*>(ws) + rows * s.n);
+    const int group = step_group(v, rows);
+    if (!group) {                                           // the row's sums first
+        const SegPlan s = score_segments(v, rows);
+        a.aux = reinterpret_cast<float*>(static_cast<Partial*>(ws) + (s.n > 1 ? rows * s.n : 0));
         distill_loss_rows(v, rows, a, ws, st);
         distill_grad_rows(v, rows, a, grad, st);
         return;
@@ -1219,14 +1405,18 @@ void launch_distill_step(const LogitsView& v, int64_t rows, const DistillList& d
     by_dtype(v.dtype, [&](auto* tp) {
         using T = std::remove_pointer_t<decltype(tp)>;
         T* out = static_cast<T*>(grad);
-        const unsigned per = 4u * (a.k + (a.tail ? (unsigned)((v.classes + 31) / 32) : 0));
-        if (wave_rows(v)) {
-            if (a.tail) hipLaunchKernelGGL((distill_step_row_kernel<T, 64, true>), dim3(blocks_of(rows, 4)), dim3(256), per * 4, st, v, rows, a, out);
-            else hipLaunchKernelGGL((distill_step_row_kernel<T, 64, false>), dim3(blocks_of(rows, 4)), dim3(256), per * 4, st, v, rows, a, out);
-        } else {
-            if (a.tail) hipLaunchKernelGGL((distill_step_row_kernel<T, 256, true>), dim3((unsigned)rows), dim3(256), per, st, v, rows, a, out);
-            else hipLaunchKernelGGL((distill_step_row_kernel<T, 256, false>), dim3((unsigned)rows), dim3(256), per, st, v, rows, a, out);
-        }
+        const int n = (int)v.classes;
+        by_bool(a.tail, [&](auto tail) {
+            constexpr bool TAIL = decltype(tail)::value;
+            if (group == 64)
+                hipLaunchKernelGGL((distill_step_kernel<T, 64, TAIL>), dim3(blocks_of(rows, 4)), dim3(256), 16u * (3 * a.k + (TAIL ? mark_words<T, 64>(n) : 0)), st, v, rows, a, out);
+            else if (group == 256)
+                hipLaunchKernelGGL((distill_step_kernel<T, 256, TAIL>), dim3((unsigned)rows), dim3(256), 4u * (3 * a.k + (TAIL ? mark_words<T, 256>(n) : 0)), st, v, rows, a, out);
+            else if (group == 512)
+                hipLaunchKernelGGL((distill_step_kernel<T, 512, TAIL>), dim3((unsigned)rows), dim3(512), 4u * (3 * a.k + (TAIL ? mark_words<T, 512>(n) : 0)), st, v, rows, a, out);
+            else
+                hipLaunchKernelGGL((distill_step_kernel<T, 1024, TAIL>), dim3((unsigned)rows), dim3(1024), 4u * (3 * a.k + (TAIL ? mark_words<T, 1024>(n) : 0)), st, v, rows, a, out);
+        });
     });
 }
 
