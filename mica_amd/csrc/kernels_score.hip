@@ -37,9 +37,19 @@ template <> __device__ __forceinline__ float from_f32<float>(float x) { return x
 template <> __device__ __forceinline__ bf16_t from_f32<bf16_t>(float x) { return {__builtin_bit_cast(unsigned short, (__bf16)x)}; }      // to nearest, ties to even
 template <> __device__ __forceinline__ f16_t from_f32<f16_t>(float x) { return {(_Float16)x}; }
 
+// Which accesses bypass the caches (ONCE), by the size of the logits.  ONCE_STORE beyond 64 MB: what a gradient's stores would push out is
+// worth more to whoever runs next (gradient of 4096 x 32000 bf16 123 -> 104 us).  ONCE_BOTH, where the kernel does not read a row twice,
+// beyond 256 MB, the Infinity Cache, if all rows begin on 16 bytes: 4096 x 128000 bf16 200 -> 175 us, their gradient 402 -> 384; at 262 MB
+// nothing gained, and lost where a later pass would have found the rows cached, or where neighbouring lanes share the lines of unaligned
+// vectors (2048 x 50001 f16 66 -> 75 us).
+enum { ONCE_NONE, ONCE_STORE, ONCE_BOTH };
 template <typename T> struct Vec { static constexpr int N = 16 / sizeof(T); };
 
 template <typename T> __device__ __forceinline__ uint4v load_raw(const T* p) { return *reinterpret_cast<const uint4u*>(p); }
+template <bool ONCE, typename T> __device__ __forceinline__ uint4v load_raw(const T* p) {
+    if constexpr (ONCE) return __builtin_nontemporal_load(reinterpret_cast<const uint4u*>(p));
+    else return load_raw(p);
+}
 // (the whole vector is cast at once: a bit cast of one element of an ext_vector reads element 0)
 __device__ __forceinline__ void unpack(uint4v q, float (&f)[4], float*) {
     const floatx4 v = __builtin_bit_cast(floatx4, q);
@@ -79,11 +89,12 @@ template <typename T> __device__ __forceinline__ uint4v raw_neg_inf();
 template <> __device__ __forceinline__ uint4v raw_neg_inf<float>() { return 0xFF800000u; }
 template <> __device__ __forceinline__ uint4v raw_neg_inf<bf16_t>() { return 0xFF80FF80u; }
 template <> __device__ __forceinline__ uint4v raw_neg_inf<f16_t>() { return 0xFC00FC00u; }
-template <typename T, int N> __device__ __forceinline__ void store_vec(T* p, const float (&f)[N]) {
+template <bool ONCE, typename T, int N> __device__ __forceinline__ void store_vec(T* p, const float (&f)[N]) {
     struct alignas(16) { T t[N]; } o;
 #pragma unroll
     for (int j = 0; j < N; ++j) o.t[j] = from_f32<T>(f[j]);
-    *reinterpret_cast<uint4u*>(p) = __builtin_bit_cast(uint4v, o);
+    if constexpr (ONCE) __builtin_nontemporal_store(__builtin_bit_cast(uint4v, o), reinterpret_cast<uint4u*>(p));
+    else *reinterpret_cast<uint4u*>(p) = __builtin_bit_cast(uint4v, o);
 }
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -308,119 +319,211 @@ __device__ __forceinline__ ListPos list_pos(const LogitsView& v, RowPos p, int64
 // ========================================================================================================================================
 constexpr int UNROLL = 4;
 
-// Streams the n classes at z: f(raw[UNROLL], i) for UNROLL 16-byte vectors of this thread at a time (vector i + u G is the u-th), with the
-// next ones on their way; then g(values[N], vector) for each vector of the rest, classes beyond n = -inf.  All threads of the group make
-// the same calls, g also for vectors that lie beyond n.
-template <typename T, int G, typename F, typename H> __device__ __forceinline__ void stream_row(const T* __restrict__ z, int n, int tid, F&& f, H&& g) {
+// Vector `vec` of the n classes at z, raw: the last one, if n does not fill it, is read from z + n - N with the classes in front of it
+// dropped (they lie in this row or, in a later segment, in the one before), so its class nfull N + i is element i + edge_shift.
+template <typename T> __device__ __forceinline__ int edge_shift(int n, int vec) {
     constexpr int N = Vec<T>::N;
-    const int nfull = n / N, rounds = nfull / (UNROLL * G);
-    if (rounds > 0) {
-        uint4v q[UNROLL];
+    return vec == n / N ? N - n % N : 0;
+}
+template <typename T> __device__ __forceinline__ uint4v load_vec(const T* __restrict__ z, int n, int vec) {
+    constexpr int N = Vec<T>::N;
+    uint4v q = raw_neg_inf<T>();
+    if (vec < n / N) q = load_raw(z + (int64_t)vec * N);
+    else if (vec * N < n) q = raw_drop(load_raw(z + (n - N)), (1u << (N - n % N)) - 1u, (T*)nullptr);
+    return q;
+}
+// Streams the n classes at z: f(raw[U], i) for U 16-byte vectors of this thread at a time (vector i + u G is the u-th), with the
+// next ones on their way; the last, partial round vector by vector: g(values[N], vector), classes beyond n = -inf.  All threads of the
+// group make the same calls, g also for vectors that lie beyond n.
+template <typename T, int G, int U, int ONCE, typename F, typename H> __device__ __forceinline__ void stream_row(const T* __restrict__ z, int n, int tid, F&& f, H&& g) {
+    constexpr int N = Vec<T>::N;
+    const int rounds = n / N / (U * G);                    // of whole vectors only
+    const bool more = rounds * U * G * N < n;
+    uint4v q[U];
+    const auto load = [&](int it) {
+        if (it < rounds) {
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) q[u] = load_raw(z + (int64_t)(tid + u * G) * N);
-        for (int it = 1; it < rounds; ++it) {
-            uint4v next[UNROLL];
+            for (int u = 0; u < U; ++u) q[u] = load_raw<ONCE == ONCE_BOTH>(z + (int64_t)(tid + (it * U + u) * G) * N);
+        } else if (more) {
 #pragma unroll
-            for (int u = 0; u < UNROLL; ++u) next[u] = load_raw(z + (int64_t)(tid + (it * UNROLL + u) * G) * N);
-            f(q, tid + (it - 1) * UNROLL * G);
-#pragma unroll
-            for (int u = 0; u < UNROLL; ++u) q[u] = next[u];
+            for (int u = 0; u < U; ++u) q[u] = load_vec(z, n, tid + (it * U + u) * G);
         }
-        f(q, tid + (rounds - 1) * UNROLL * G);
+    };
+    load(0);
+    for (int it = 0; it < rounds; ++it) {
+        uint4v now[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) now[u] = q[u];
+        load(it + 1);
+        f(now, tid + it * U * G);
     }
-    for (int i = rounds * UNROLL * G; i * N < n; i += G) {
-        const int vec = i + tid;
-        float v[N];
-        if (vec < nfull) unpack(load_raw(z + (int64_t)vec * N), v, (T*)nullptr);
-        else {
+    if (more) {
 #pragma unroll
-            for (int j = 0; j < N; ++j) v[j] = vec * N + j < n ? to_f32(z[vec * N + j]) : -INFINITY;
+        for (int u = 0; u < U; ++u) {
+            const int i = (rounds * U + u) * G;
+            if (i * N >= n) break;                              // of the whole group
+            float v[N];
+            unpack(q[u], v, (T*)nullptr);
+            g(v, i + tid);
         }
-        g(v, vec);
     }
 }
 
-// The K <= 64 largest of a group's row.  While streaming, every thread notes its largest value and the vector that held it first.  The
-// K-th largest of these (value, position) pairs bounds the K-th largest element from below, so only the threads at or above the bound
-// can own one of the K: their vectors are read once more (K / G of the row, from cache) and what passes the bound is merged, 64 keys at
-// a time, into a sorted list that each wave holds one key per lane.  Exact for any data; ties and -inf order by index.
+// The K <= 64 largest of a group's row.  While streaming, every thread notes its largest value and the vector that held it first.  Of
+// these (value, position) pairs each wave takes its ceil(K / waves)-th largest; the smallest of those bounds the K-th largest element
+// from below, so only threads at or above the bound can own one of the K.  A long row is noted in PARTS stretches, and only the stretches
+// at or above the bound are read once more (about K / (PARTS G) of the row) and what passes the bound is sorted, one key per lane.  More than 64 pass only in unusual data (many equal values, everything
+// large in one place); then every wave merges its share, 64 keys at a time, into a sorted list.  Exact for any data; ties and -inf order
+// by index.
 struct TopScratch {             // LDS of one wave
     u64 list[64];
     u64 buf[128];
 };
-// the merged top 64 of the block's waves; `list` descending per wave
-template <int NW> __device__ __forceinline__ u64 merge_waves(u64 list, TopScratch* sc, int w, int lane) {
-    sc[w].list[lane] = list;
-    __syncthreads();
-    list = sc[0].list[lane];
+struct TopShared { u64 bound[4]; int owners_n, passed; };
+constexpr int PARTS = 4;
+// what a thread notes: its best of each stretch (per_part rounds of UNROLL vectors; the last one takes the rest)
+struct TopNote {
+    u64 key[PARTS];
+    float best;
+    int best_at, part, left;
+    bool any;
+    __device__ __forceinline__ void start(int per_part) {
 #pragma unroll
-    for (int i = 1; i < NW; ++i) list = merge_top64(list, sc[i].list[63 - lane], lane);
-    return list;
+        for (int i = 0; i < PARTS; ++i) key[i] = 0;
+        best = -INFINITY;
+        best_at = part = 0;
+        left = per_part;
+        any = false;
+    }
+    __device__ __forceinline__ void see(float vm, int at) {
+        if (vm > best || !any) { best = vm; best_at = at; }
+        any = true;
+    }
+    __device__ __forceinline__ void close() {                   // the stretch ends
+        const u64 k = any ? make_key(order_key(best), (unsigned)best_at) : 0;
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) key[i] = i == part ? k : key[i];
+        best = -INFINITY;
+        any = false;
+    }
+    __device__ __forceinline__ void round_done(int per_part) {  // the same in all threads of a group
+        if (--left == 0 && part < PARTS - 1) {
+            close();
+            ++part;
+            left = per_part;
+        }
+    }
+};
+template <typename T, int G> __device__ __forceinline__ int rounds_per_part(int n) {
+    const int rounds = n / Vec<T>::N / (UNROLL * G);
+    return rounds < PARTS ? 1 : rounds / PARTS;
 }
 template <typename T, int G>
-__device__ __forceinline__ u64 group_top(const T* __restrict__ z, int n, unsigned index0, int k, float best, int best_at, bool any, TopScratch* sc,
-                                         int* owners, int* nown) {
+__device__ __forceinline__ u64 group_top(const T* __restrict__ z, int n, unsigned index0, int k, const TopNote& note, TopScratch* sc, int* owners,
+                                         TopShared* sh) {
     constexpr int N = Vec<T>::N, NW = G / 64;
     const int tid = G == 64 ? (threadIdx.x & 63) : threadIdx.x, lane = threadIdx.x & 63, w = G == 64 ? 0 : threadIdx.x >> 6;
-    const u64 mine = any ? make_key(order_key(best), (unsigned)best_at) : 0;
-    u64 sorted = sort64<true>(mine, lane);
-    if (NW > 1) {
-        if (threadIdx.x == 0) *nown = 0;
-        sorted = merge_waves<NW>(sorted, sc, w, lane);
-    }
-    const u64 bound = lane_key(sorted, k - 1);
+    u64 mine = note.key[0];
+#pragma unroll
+    for (int i = 1; i < PARTS; ++i) mine = note.key[i] > mine ? note.key[i] : mine;
+    u64 bound = lane_key(sort64<true>(mine, lane), (k + NW - 1) / NW - 1);
     int count;
     if (NW > 1) {
-        if (any && mine >= bound) owners[atomicAdd(nown, 1)] = tid;      // the order of the owners does not change the result
+        if (lane == 0) sh->bound[w] = bound;
+        if (threadIdx.x == 0) sh->owners_n = sh->passed = 0;
         __syncthreads();
-        count = *nown;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) bound = sh->bound[i] < bound ? sh->bound[i] : bound;
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i)                         // the order of the owners does not change the result
+            if (note.key[i] != 0 && note.key[i] >= bound) owners[atomicAdd(&sh->owners_n, 1)] = i * G + tid;
+        __syncthreads();
+        count = sh->owners_n;
     } else {
-        const u64 b = __ballot(any && mine >= bound);
-        if (any && mine >= bound) owners[__popcll(b & ((1ull << lane) - 1))] = tid;
-        wave_sync();
-        count = __popcll(b);
-    }
-    const int nvec = (n + N - 1) / N, per = (nvec + G - 1) / G;
-    const int total = count * per;
-    u64 list = 0, floor_key = 0;
-    int pending = 0;
-    for (int p0 = 0; p0 < total; p0 += G) {
-        const int p = p0 + tid;
-        const int vec = p < total ? owners[p % count] + (p / count) * G : nvec;
-        float v[N];
-        if ((vec + 1) * N <= n) unpack(load_raw(z + (int64_t)vec * N), v, (T*)nullptr);
-        else {
+        count = 0;
 #pragma unroll
-            for (int j = 0; j < N; ++j) v[j] = vec * N + j < n ? to_f32(z[vec * N + j]) : 0.f;
+        for (int i = 0; i < PARTS; ++i) {
+            const bool own = note.key[i] != 0 && note.key[i] >= bound;
+            const u64 b = __ballot(own);
+            if (own) owners[count + __popcll(b & ((1ull << lane) - 1))] = i * G + tid;
+            count += __popcll(b);
         }
+        wave_sync();
+    }
+    const int nvec = (n + N - 1) / N, rounds = nvec / (UNROLL * G) + 1, per_part = rounds_per_part<T, G>(n);
+    // the longest stretch, in vectors of one thread: the last one
+    const int per = (rounds - (PARTS - 1) * per_part > per_part ? rounds - (PARTS - 1) * per_part : per_part) * UNROLL;
+    const int total = count * per;
+    // take(passes, key), by whole waves, for every class the owners hold
+    const auto scan = [&](auto&& take) {
+        for (int p0 = 0; p0 < total; p0 += G) {
+            const int p = p0 + tid;
+            int vec = nvec;
+            if (p < total) {
+                const int own = owners[p % count], part = own / G, i = p / count;       // the i-th vector of the stretch
+                if (part == PARTS - 1 || i < per_part * UNROLL) vec = own % G + (part * per_part * UNROLL + i) * G;
+                if (vec > nvec) vec = nvec;
+            }
+            const int shift = edge_shift<T>(n, vec);
+            float v[N];
+            unpack(load_vec(z, n, vec), v, (T*)nullptr);
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const int at = vec * N + j;
-            const unsigned o = order_key(v[j]);
-            const u64 key = make_key(o, (unsigned)at);
-            const bool pass = at < n && make_key(o, (unsigned)(vec * N)) >= bound && key > floor_key;
+            for (int j = 0; j < N; ++j) {
+                const int at = vec * N + j - shift;
+                const unsigned o = order_key(v[j]);
+                take(vec < nvec && j >= shift && make_key(o, (unsigned)(vec * N)) >= bound, make_key(o, (unsigned)at));
+            }
+        }
+    };
+    u64 list = 0;
+    bool few = false;
+    if (NW > 1) {
+        scan([&](bool pass, u64 key) {
+            if (pass) {
+                const int i = atomicAdd(&sh->passed, 1);
+                if (i < 64) sc[0].buf[i] = key;
+            }
+        });
+        __syncthreads();
+        const int passed = sh->passed;
+        few = passed <= 64;
+        if (few) {
+            if (w == 0) list = sort64<true>(lane < passed ? sc[0].buf[lane] : 0, lane);
+        } else {
+            __syncthreads();                                    // buf is about to be written again
+        }
+    }
+    if (!few) {
+        u64 floor_key = 0;
+        int pending = 0;
+        scan([&](bool pass0, u64 key) {
+            const bool pass = pass0 && key > floor_key;
             const u64 b = __ballot(pass);
-            if (b == 0) continue;
+            if (b == 0) return;
             if (pass) sc[w].buf[pending + __popcll(b & ((1ull << lane) - 1))] = key;
             pending += __popcll(b);
             wave_sync();
             if (pending >= 64) {
-                const u64 take = sc[w].buf[lane], rest = sc[w].buf[64 + lane];
+                const u64 now = sc[w].buf[lane], rest = sc[w].buf[64 + lane];
                 wave_sync();
                 sc[w].buf[lane] = rest;
                 wave_sync();
                 pending -= 64;
-                list = merge_top64(list, sort64<false>(take, lane), lane);
+                list = merge_top64(list, sort64<false>(now, lane), lane);
                 floor_key = lane_key(list, k - 1);
+            }
+        });
+        if (pending > 0) list = merge_top64(list, sort64<false>(lane < pending ? sc[w].buf[lane] : 0, lane), lane);
+        if (NW > 1) {
+            sc[w].list[lane] = list;
+            __syncthreads();
+            if (w == 0) {
+#pragma unroll
+                for (int i = 1; i < NW; ++i) list = merge_top64(list, sc[i].list[63 - lane], lane);
             }
         }
     }
-    if (pending > 0) list = merge_top64(list, sort64<false>(lane < pending ? sc[w].buf[lane] : 0, lane), lane);
-    if (NW > 1) {
-        __syncthreads();
-        list = merge_waves<NW>(list, sc, w, lane);
-    }
-    // classes are numbered within the segment so far
+    // (of wave 0) classes are numbered within the segment so far
     return list == 0 ? 0 : ((list & 0xFFFFFFFF00000000ull) | (0xFFFFFFFFu - (key_index(list) + index0)));
 }
 
@@ -467,14 +570,14 @@ __device__ __forceinline__ void write_top(const ScoreOut& o, const LogitsView& v
     }
 }
 
-template <typename T, int G, bool TOP>
+template <typename T, int G, bool TOP, int ONCE>
 __global__ __launch_bounds__(256) void score_row_kernel(LogitsView v, int64_t rows, ScoreOut o, int segments, int seg_len, Partial* __restrict__ part,
                                                         u64* __restrict__ part_top) {
     constexpr int N = Vec<T>::N, NW = G / 64, GROUPS = 256 / G;
     __shared__ Partial waves[4];
     __shared__ TopScratch top_sc[TOP ? 4 : 1];
-    __shared__ int owners[TOP ? 256 : 1];
-    __shared__ int nown;
+    __shared__ int owners[TOP ? 256 * PARTS : 1];
+    __shared__ TopShared top_sh;
     const int g = threadIdx.x / G, tid = threadIdx.x % G, lane = threadIdx.x & 63;
     const int64_t item = (int64_t)blockIdx.x * GROUPS + g;
     if (item >= rows * segments) return;                   // whole waves; with G = 256 the grid is exact
@@ -485,16 +588,10 @@ __global__ __launch_bounds__(256) void score_row_kernel(LogitsView v, int64_t ro
     const int first = seg * seg_len;
     const int n = (int)(v.classes - first < seg_len ? v.classes - first : seg_len);
     Online on;
-    float best = -INFINITY;
-    int best_at = 0;
-    bool any = false;
-    const auto note = [&](float vm, int vec) {
-        if (TOP) {
-            if (vm > best || !any) { best = vm; best_at = vec * N; }
-            any = true;
-        }
-    };
-    stream_row<T, G>(
+    TopNote note;
+    const int per_part = rounds_per_part<T, G>(n);
+    if (TOP) note.start(per_part);
+    stream_row<T, G, UNROLL, ONCE>(
         z + first, n, tid,
         [&](const uint4v(&q)[UNROLL], int i) {
             float f[UNROLL * N], vm = -INFINITY;
@@ -503,21 +600,25 @@ __global__ __launch_bounds__(256) void score_row_kernel(LogitsView v, int64_t ro
                 float x[N];
                 unpack(q[u], x, (T*)nullptr);
                 const float mu = max_of(x);
-                note(mu, i + u * G);
+                if (TOP) note.see(mu, (i + u * G) * N);
                 vm = fmaxf(vm, mu);
 #pragma unroll
                 for (int j = 0; j < N; ++j) f[u * N + j] = x[j];
             }
+            if (TOP) note.round_done(per_part);
             on.add<UNROLL * N, true>(f, vm, o.c);
         },
         [&](const float(&f)[N], int vec) {
             const float vm = max_of(f);
-            if (vec * N < n) note(vm, vec);
+            if (TOP && vec * N < n) note.see(vm, vec * N);
             on.add<N, true>(f, vm, o.c);
         });
     on = group_join<G>(on, o.c, waves);
     u64 key = 0;
-    if (TOP) key = group_top<T, G>(z + first, n, (unsigned)first, o.top, best, best_at, any, NW == 1 ? &top_sc[g] : top_sc, &owners[g * G], &nown);
+    if (TOP) {
+        note.close();
+        key = group_top<T, G>(z + first, n, (unsigned)first, o.top, note, NW == 1 ? &top_sc[g] : top_sc, &owners[g * G * PARTS], &top_sh);
+    }
     if (segments == 1) {
         if (tid < 64) {
             const double log_s = log_sum(on.m, on.s, o.c);        // s is about 1 or more unless the row is empty (0) or holds NaN
@@ -622,14 +723,14 @@ __device__ __forceinline__ float grad_value(const RowGrad& g, float z, float c) 
 }
 
 // what a block of the gradient kernels covers: G threads x UNROLL vectors of one row
-template <typename T, int G, typename F>
+template <typename T, int G, int ONCE, typename F>
 __device__ __forceinline__ void map_chunk(const T* __restrict__ z, T* __restrict__ out, int first, int64_t classes, int tid, F&& f) {
     constexpr int N = Vec<T>::N;
     uint4v q[UNROLL];
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
         const int64_t at = first + (int64_t)(tid + u * G) * N;
-        if (at + N <= classes) q[u] = load_raw(z + at);
+        if (at + N <= classes) q[u] = load_raw<ONCE == ONCE_BOTH>(z + at);
     }
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
@@ -639,7 +740,7 @@ __device__ __forceinline__ void map_chunk(const T* __restrict__ z, T* __restrict
             unpack(q[u], v, (T*)nullptr);
 #pragma unroll
             for (int j = 0; j < N; ++j) v[j] = f(v[j], at + j);
-            store_vec(out + at, v);
+            store_vec<ONCE != ONCE_NONE>(out + at, v);
         } else {
             for (int j = 0; j < N; ++j)
                 if (at + j < classes) out[at + j] = from_f32<T>(f(to_f32(z[at + j]), at + j));
@@ -647,7 +748,7 @@ __device__ __forceinline__ void map_chunk(const T* __restrict__ z, T* __restrict
     }
 }
 
-template <typename T, int G>
+template <typename T, int G, int ONCE>
 __global__ __launch_bounds__(256) void score_grad_row_kernel(LogitsView v, int64_t rows, ScoreGrad o, int chunks, T* __restrict__ grad) {
     constexpr int GROUPS = 256 / G, CHUNK = G * UNROLL * Vec<T>::N;
     const int tid = threadIdx.x % G;
@@ -657,7 +758,7 @@ __global__ __launch_bounds__(256) void score_grad_row_kernel(LogitsView v, int64
     const int first = chunks == 1 ? 0 : (int)(item % chunks) * CHUNK;
     const RowGrad g = row_grad(o, v.classes, r);
     const T* z = static_cast<const T*>(v.p) + row_start(v, row_pos(v, r));
-    map_chunk<T, G>(z, grad + r * v.classes, first, v.classes, tid,
+    map_chunk<T, G, ONCE>(z, grad + r * v.classes, first, v.classes, tid,
                     [&](float x, int64_t at) { return grad_value(g, x, o.c) + (at == g.token ? g.at_token : 0.f); });
 }
 
@@ -678,10 +779,7 @@ struct DistillArgs {
 // A row's gradient: factor * e^{y - ref} where a class is not listed, mass * e^{y - lse} - sum p at a listed one, times T and the
 // upstream gradient.  (tail: ref is the log sum of the classes that are not listed and factor = mass q_rest - r, so that nothing
 // overflows where q_rest is tiny; else ref = lse, factor = mass.)
-struct RowDistill { float loss, ref, factor, lse, mass, norm; };
-
 // The row's list in LDS: index (unused entries -1, no class: INT_MAX), log probability, logit.  Loaded by one wave.
-constexpr int SLOTS = 4;                                        // entries per lane of that wave: 256 in all
 struct ListLds { int* i; float* t; float* z; };
 constexpr unsigned LIST_BYTES = 12;                             // of LDS per entry
 __device__ __forceinline__ ListLds list_lds(int* base, int k) { return {base, reinterpret_cast<float*>(base + k), reinterpret_cast<float*>(base + 2 * k)}; }
@@ -695,20 +793,20 @@ __device__ __forceinline__ void list_load(const DistillArgs& a, ListPos l, const
         d.z[k] = v < 0 || v >= classes ? -INFINITY : to_f32(z[v]);
     }
 }
-// A bit per class, laid out as the stream reads it: class v of vector vec = v / N is bit (vec / G % UNROLL) * 8 + v % N of word
-// (vec / (UNROLL G)) G + vec % G, one word for the UNROLL vectors a thread takes at a time.
-template <typename T, int G> __host__ __device__ constexpr int mark_words(int n) {
-    return ((n + Vec<T>::N - 1) / Vec<T>::N + UNROLL * G - 1) / (UNROLL * G) * G;
+// A bit per class, laid out as the stream reads it: class v of vector vec = v / N is bit (vec / G % U) * 8 + v % N of word
+// (vec / (U G)) G + vec % G, one word for the U vectors a thread takes at a time.
+template <typename T, int G, int U = UNROLL> __host__ __device__ constexpr int mark_words(int n) {
+    return ((n + Vec<T>::N - 1) / Vec<T>::N + U * G - 1) / (U * G) * G;
 }
-template <typename T, int G> __device__ __forceinline__ void mark_listed(const int* idx, int k, int first, int n, unsigned* bits, int tid) {
+template <typename T, int G, int U = UNROLL> __device__ __forceinline__ void mark_listed(const int* idx, int k, int first, int n, unsigned* bits, int tid) {
     constexpr int N = Vec<T>::N;
-    for (int i = tid; i < mark_words<T, G>(n); i += G) bits[i] = 0;
+    for (int i = tid; i < mark_words<T, G, U>(n); i += G) bits[i] = 0;
     group_sync<G>();
     for (int i = tid; i < k; i += G) {
         const int v = idx[i] - first;
         if (idx[i] >= 0 && v >= 0 && v < n) {
             const int vec = v / N;
-            atomicOr(&bits[vec / (UNROLL * G) * G + vec % G], 1u << (vec / G % UNROLL * 8 + v % N));
+            atomicOr(&bits[vec / (U * G) * G + vec % G], 1u << (vec / G % U * 8 + v % N));
         }
     }
     group_sync<G>();
@@ -720,17 +818,17 @@ template <int N> __device__ __forceinline__ void drop_listed(float (&f)[N], unsi
     }
 }
 // the online sums of the classes of a segment, without the listed ones if TAIL
-template <typename T, int G, bool TAIL>
+template <typename T, int G, bool TAIL, int U, int ONCE>
 __device__ __forceinline__ Online distill_stream(const T* __restrict__ z, int n, int tid, const unsigned* bits, float c) {
     constexpr int N = Vec<T>::N;
     Online on;
-    stream_row<T, G>(
+    stream_row<T, G, U, ONCE>(
         z, n, tid,
-        [&](const uint4v(&q)[UNROLL], int i) {
-            const unsigned b = TAIL ? bits[i / UNROLL / G * G + tid] : 0u;
-            float f[UNROLL * N], vm = -INFINITY;
+        [&](const uint4v(&q)[U], int i) {
+            const unsigned b = TAIL ? bits[i / U / G * G + tid] : 0u;
+            float f[U * N], vm = -INFINITY;
 #pragma unroll
-            for (int u = 0; u < UNROLL; ++u) {
+            for (int u = 0; u < U; ++u) {
                 float x[N];
                 unpack(q[u], x, (T*)nullptr);
                 if (TAIL) drop_listed(x, (b >> (8 * u)) & 0xFFu);
@@ -738,116 +836,132 @@ __device__ __forceinline__ Online distill_stream(const T* __restrict__ z, int n,
 #pragma unroll
                 for (int j = 0; j < N; ++j) f[u * N + j] = x[j];
             }
-            on.add<UNROLL * N, false>(f, vm, c);
+            on.add<U * N, false>(f, vm, c);
         },
         [&](const float(&f0)[N], int vec) {
             float f[N];
 #pragma unroll
             for (int j = 0; j < N; ++j) f[j] = f0[j];
-            if (TAIL && vec * N < n) drop_listed(f, (bits[vec / (UNROLL * G) * G + vec % G] >> (vec / G % UNROLL * 8)) & 0xFFu);
+            if (TAIL && vec * N < n) drop_listed(f, ((bits[vec / (U * G) * G + vec % G] >> (vec / G % U * 8)) & 0xFFu) << edge_shift<T>(n, vec));
             on.add<N, false>(f, max_of(f), c);
         });
     return on;
 }
 
-// The row's loss and what its gradient needs, from the sums over all classes, or over the classes that are not listed (tail).  One
-// wave; every lane gets the result.  What cancels is combined in float64: 1 - sum p, the terms of a good
-// student, log q_rest = -log(1 + listed sum / rest sum).
-__device__ __forceinline__ RowDistill distill_finish(const DistillArgs& a, ListLds d, float m, float s, int lane) {
-    struct { int i[SLOTS]; float t[SLOTS], z[SLOTS]; } l;
-#pragma unroll
-    for (int e = 0; e < SLOTS; ++e) {
-        const int k = lane + 64 * e;
-        l.i[e] = k < a.k ? d.i[k] : -1;
-        l.t[e] = k < a.k ? d.t[k] : -INFINITY;
-        l.z[e] = k < a.k ? d.z[k] : -INFINITY;
-    }
-    RowDistill o;
+// What a row's list says by itself: one wave, in every lane.
+struct ListStats {
+    double mass;        // sum p: of the renormalised list 1, or 0 if no entry has any; tail: sum of e^t
+    double norm;        // log sum of the values (renormalised), 0 (tail)
+    double log_sl;      // (tail) log of the listed classes' sum relative to zmax, every class once; -inf: none
+    float zmax;
+    int bad;            // an index that is no class
+};
+__device__ __forceinline__ ListStats list_stats(const DistillArgs& a, ListLds d, int lane) {
+    ListStats o;
     bool bad = false;
     float tmax = -INFINITY, zmax = -INFINITY;
-#pragma unroll
-    for (int e = 0; e < SLOTS; ++e) {
-        bad |= l.i[e] == 0x7FFFFFFF;
-        tmax = fmaxf(tmax, l.t[e]);
-        zmax = fmaxf(zmax, l.z[e]);
+    for (int k = lane; k < a.k; k += 64) {
+        bad |= d.i[k] == 0x7FFFFFFF;
+        tmax = fmaxf(tmax, d.t[k]);
+        zmax = fmaxf(zmax, d.z[k]);
     }
-    bad = __any(bad);
-    const double log_m = log_sum(m, s, a.c);                    // log of the streamed sum relative to m
-    const bool have_rest = !(s == 0.f);                         // NaN counts
-    double norm = 0.0, mass = 1.0, rest = 0.0, log_q_rest = 0.0, lse_rest = 0.0;
-    double M = m, log_s = log_m;                                // maximum and log sum of all classes
+    o.bad = __any(bad);
+    o.zmax = zmax = wave_max(zmax);
+    o.log_sl = -INFINITY;
     if (!a.tail) {
         tmax = wave_max(tmax);
         double sum = 0.0;
-#pragma unroll
-        for (int e = 0; e < SLOTS; ++e)
-            if (l.i[e] >= 0) sum += tmax == -INFINITY ? (l.t[e] != l.t[e] ? (double)l.t[e] : 0.0) : exp((double)l.t[e] - tmax);
+        for (int k = lane; k < a.k; k += 64)
+            if (d.i[k] >= 0) sum += tmax == -INFINITY ? (d.t[k] != d.t[k] ? (double)d.t[k] : 0.0) : exp((double)d.t[k] - tmax);
         sum = wave_sum(sum);
-        norm = sum == 0.0 ? -INFINITY : (tmax == -INFINITY ? sum : tmax + log(sum));
-        mass = sum == 0.0 ? 0.0 : 1.0;
+        o.norm = sum == 0.0 ? -INFINITY : (tmax == -INFINITY ? sum : tmax + log(sum));
+        o.mass = sum == 0.0 ? 0.0 : 1.0;
     } else {
-        zmax = wave_max(zmax);
         double sl = 0.0, P = 0.0;
-#pragma unroll
-        for (int e = 0; e < SLOTS; ++e) {
-            if (l.i[e] < 0) continue;
-            P += exp((double)l.t[e]);
+        for (int k = lane; k < a.k; k += 64) {
+            const int i = d.i[k];
+            if (i < 0) continue;
+            P += exp((double)d.t[k]);
             bool again = false;
-            for (int j = 0; j < lane + 64 * e; ++j) again |= d.i[j] == l.i[e];
-            if (!again) sl += zmax == -INFINITY ? (l.z[e] != l.z[e] ? (double)l.z[e] : 0.0) : (double)exp2_hw((l.z[e] - zmax) * a.c);
+            for (int j = 0; j < k; ++j) again |= d.i[j] == i;
+            if (!again) sl += zmax == -INFINITY ? (d.z[k] != d.z[k] ? (double)d.z[k] : 0.0) : (double)exp2_hw((d.z[k] - zmax) * a.c);
         }
-        sl = wave_sum(sl);
-        P = wave_sum(P);
-        rest = have_rest ? (P < 1.0 ? 1.0 - P : 0.0) : 0.0;
-        mass = P + rest;
+        o.log_sl = log(wave_sum(sl));
+        o.mass = wave_sum(P);
+        o.norm = 0.0;
+    }
+    return o;
+}
+// The row's scalars from its list and the sums over all classes, or over those that are not listed (tail); any thread.  What cancels is
+// combined in float64: 1 - sum p, log q_rest = -log(1 + listed sum / rest sum).
+struct RowScalars { double M, log_s, rest, log_q_rest, mass; float ref, factor, lse; };     // M, log_s: maximum and log sum of all classes
+__device__ __forceinline__ RowScalars row_scalars(const DistillArgs& a, const ListStats& l, float m, float s) {
+    RowScalars o;
+    const double log_m = log_sum(m, s, a.c);                    // log of the streamed sum relative to m
+    o.M = m;
+    o.log_s = log_m;
+    o.rest = o.log_q_rest = 0.0;
+    o.mass = l.mass;
+    const bool have_rest = !(s == 0.f);                         // NaN counts
+    double lse_rest = 0.0;
+    if (a.tail) {
+        o.rest = have_rest && l.mass < 1.0 ? 1.0 - l.mass : 0.0;
+        o.mass += o.rest;
         lse_rest = (double)m * a.inv_t + log_m;
-        if (!have_rest) { M = zmax; log_s = log(sl); }
-        else if (sl != 0.0) {
-            M = fmaxf(m, zmax);
-            const double u = ((double)zmax - m) * a.inv_t + log(sl) - log_m;      // log of (listed sum / rest sum)
-            log_q_rest = -(u > 700.0 ? u : log1p(exp(u)));
-            log_s = ((double)m - M) * a.inv_t + log_m - log_q_rest;
+        if (!have_rest) { o.M = l.zmax; o.log_s = l.log_sl; }
+        else if (l.log_sl != -INFINITY) {
+            o.M = fmaxf(m, l.zmax);
+            const double u = ((double)l.zmax - m) * a.inv_t + l.log_sl - log_m;      // log of (listed sum / rest sum)
+            o.log_q_rest = -(u > 700.0 ? u : log1p(exp(u)));
+            o.log_s = ((double)m - o.M) * a.inv_t + log_m - o.log_q_rest;
         }
     }
-    const bool empty = M == -INFINITY;
+    o.lse = s != s ? NAN : (o.M == -INFINITY ? -INFINITY : (float)(o.M * a.inv_t + o.log_s));
+    if (a.tail) {
+        o.ref = have_rest ? (float)lse_rest : 0.f;
+        o.factor = have_rest ? (float)(o.mass * exp(o.log_q_rest) - o.rest) : 0.f;
+    } else {
+        o.ref = o.lse;
+        o.factor = (float)o.mass;
+    }
+    if (l.bad || s != s) o.factor = NAN;                        // an invalid entry shows in the gradient too
+    return o;
+}
+// the loss; one wave, in every lane
+__device__ __forceinline__ float row_loss(const DistillArgs& a, ListLds d, const ListStats& l, const RowScalars& o, float s, int lane) {
     double sum = 0.0;
-#pragma unroll
-    for (int e = 0; e < SLOTS; ++e) {
-        if (l.i[e] < 0) continue;
-        const double lp = (double)l.t[e] - norm;
-        const double pk = mass == 0.0 ? 0.0 : exp(lp);
-        const double lq = empty ? -INFINITY : ((double)l.z[e] - M) * a.inv_t - log_s;
+    for (int k = lane; k < a.k; k += 64) {
+        if (d.i[k] < 0) continue;
+        const double lp = (double)d.t[k] - l.norm;
+        const double pk = o.mass == 0.0 ? 0.0 : exp(lp);
+        const double lq = o.M == -INFINITY ? -INFINITY : ((double)d.z[k] - o.M) * a.inv_t - o.log_s;
         if (!(pk == 0.0)) sum += pk * (lp - lq);
     }
     sum = wave_sum(sum);
-    if (rest > 0.0) sum += rest * (log(rest) - log_q_rest);
-    if (bad || s != s) sum = NAN;
-    o.loss = (float)(sum * a.t * a.t);
-    o.lse = s != s ? NAN : (empty ? -INFINITY : (float)(M * a.inv_t + log_s));
-    o.mass = (float)mass;
-    o.norm = (float)norm;
-    if (a.tail) {
-        o.ref = have_rest ? (float)lse_rest : 0.f;
-        o.factor = have_rest ? (float)(mass * exp(log_q_rest) - rest) : 0.f;
-    } else {
-        o.ref = o.lse;
-        o.factor = o.mass;
-    }
-    if (sum != sum) o.factor = NAN;                              // an invalid entry shows in the gradient too
-    return o;
+    if (o.rest > 0.0) sum += o.rest * (log(o.rest) - o.log_q_rest);
+    return l.bad || s != s ? NAN : (float)(sum * a.t * a.t);
 }
-__device__ __forceinline__ void write_distill(const DistillArgs& a, const RowDistill& o, int64_t r, int64_t rows) {
-    const float w = a.weight ? a.weight[r] : 1.f;
-    a.loss[r] = w == 0.f ? 0.f : o.loss * w;
-    if (a.aux) {
-        a.aux[r] = o.ref;
-        a.aux[rows + r] = o.factor;
-        a.aux[2 * rows + r] = o.lse;
-        a.aux[3 * rows + r] = a.tail ? o.mass : o.norm;
+struct RowGradient { float ref, factor, lse, mass, norm; };
+// loss and aux of a row from its joined sums; one wave, the result in every lane
+__device__ __forceinline__ RowGradient finish_row(const DistillArgs& a, ListLds d, float m, float s, int64_t r, int64_t rows, int lane) {
+    const ListStats l = list_stats(a, d, lane);
+    const RowScalars o = row_scalars(a, l, m, s);
+    const float loss = row_loss(a, d, l, o, s, lane);
+    const RowGradient q{o.ref, loss != loss ? NAN : o.factor, o.lse, (float)o.mass, (float)l.norm};
+    if (lane == 0) {
+        const float w = a.weight ? a.weight[r] : 1.f;
+        a.loss[r] = w == 0.f ? 0.f : loss * w;
+        if (a.aux) {
+            a.aux[r] = q.ref;
+            a.aux[rows + r] = q.factor;
+            a.aux[2 * rows + r] = q.lse;
+            a.aux[3 * rows + r] = a.tail ? q.mass : q.norm;
+        }
     }
+    return q;
 }
 
-template <typename T, int G, bool TAIL>
+template <typename T, int G, bool TAIL, int ONCE>
 __global__ __launch_bounds__(256) void distill_row_kernel(LogitsView v, int64_t rows, DistillArgs a, int segments, int seg_len, Partial* __restrict__ part) {
     constexpr int GROUPS = 256 / G;
     extern __shared__ int dyn[];
@@ -867,14 +981,12 @@ __global__ __launch_bounds__(256) void distill_row_kernel(LogitsView v, int64_t 
     if (tid < 64) list_load(a, list_pos(v, p, r, a.k), z, v.classes, lane, list);
     group_sync<G>();
     if (TAIL) mark_listed<T, G>(list.i, a.k, first, n, bits, tid);
-    const Online on = group_join<G>(distill_stream<T, G, TAIL>(z + first, n, tid, bits, a.c), a.c, waves);
+    const Online on = group_join<G>(distill_stream<T, G, TAIL, UNROLL, ONCE>(z + first, n, tid, bits, a.c), a.c, waves);
     if (segments > 1) {
         if (tid == 0) part[item] = {on.m, on.s, 0.f, 0.f};
         return;
     }
-    if (tid >= 64) return;
-    const RowDistill o = distill_finish(a, list, on.m, on.s, lane);
-    if (lane == 0) write_distill(a, o, r, rows);
+    if (tid < 64) (void)finish_row(a, list, on.m, on.s, r, rows, lane);
 }
 template <typename T>
 __global__ __launch_bounds__(64) void distill_join_kernel(LogitsView v, int64_t rows, DistillArgs a, int segments, const Partial* __restrict__ part) {
@@ -885,14 +997,12 @@ __global__ __launch_bounds__(64) void distill_join_kernel(LogitsView v, int64_t 
     list_load(a, list_pos(v, p, r, a.k), static_cast<const T*>(v.p) + row_start(v, p), v.classes, threadIdx.x, list);
     wave_sync();
     const Online on = join_segments(part + r * segments, segments, a.c);
-    const RowDistill o = distill_finish(a, list, on.m, on.s, threadIdx.x);
-    if (threadIdx.x == 0) write_distill(a, o, r, rows);
+    (void)finish_row(a, list, on.m, on.s, r, rows, threadIdx.x);
 }
 
 // the listed classes of [first, first + n): overwrites what the sweep wrote there; the first mention of a class writes for all of them
 template <typename T, int G>
-__device__ __forceinline__ void listed_grad(const DistillArgs& a, T* __restrict__ out, ListLds d, int64_t first, int64_t n, float lse, float mass, float norm,
-                                            float scale, int tid) {
+__device__ __forceinline__ void listed_grad(const DistillArgs& a, T* __restrict__ out, ListLds d, int64_t first, int64_t n, RowGradient q, float scale, int tid) {
     for (int k = tid; k < a.k; k += G) {
         const int i = d.i[k];
         if (i < first || i >= first + n || i < 0 || i == 0x7FFFFFFF) continue;
@@ -901,14 +1011,14 @@ __device__ __forceinline__ void listed_grad(const DistillArgs& a, T* __restrict_
         for (int j = 0; j < a.k; ++j) {
             if (d.i[j] != i) continue;
             again |= j < k;
-            p += a.tail ? expf(d.t[j]) : (norm == -INFINITY ? 0.f : expf(d.t[j] - norm));
+            p += a.tail ? expf(d.t[j]) : (q.norm == -INFINITY ? 0.f : expf(d.t[j] - q.norm));
         }
-        if (!again) out[i] = from_f32<T>(scale * (mass * exp2_hw(fmaf(d.z[k], a.c, -lse * LOG2E)) - p));
+        if (!again) out[i] = from_f32<T>(scale * (q.mass * exp2_hw(fmaf(d.z[k], a.c, -q.lse * LOG2E)) - p));
     }
 }
 __device__ __forceinline__ float unlisted_grad(float z, float ref2, float f, float c) { return f * exp2_hw(fmaf(z, c, -ref2)); }
 
-template <typename T, int G>
+template <typename T, int G, int ONCE>
 __global__ __launch_bounds__(256) void distill_grad_row_kernel(LogitsView v, int64_t rows, DistillArgs a, int chunks, T* __restrict__ grad) {
     constexpr int GROUPS = 256 / G, CHUNK = G * UNROLL * Vec<T>::N;
     extern __shared__ int dyn[];
@@ -924,123 +1034,75 @@ __global__ __launch_bounds__(256) void distill_grad_row_kernel(LogitsView v, int
     T* out = grad + r * v.classes;
     const float w = a.weight ? a.weight[r] : 1.f;
     const float scale = (a.g_loss ? a.g_loss[r] : 1.f) * w * a.t;
-    const float ref = a.aux[r], factor = a.aux[rows + r], lse = a.aux[2 * rows + r], x = a.aux[3 * rows + r];
-    const float mass = a.tail ? x : (x == -INFINITY ? 0.f : 1.f), norm = a.tail ? 0.f : x;
-    const bool none = lse == -INFINITY || w == 0.f;
-    const float ref2 = none ? 0.f : ref * LOG2E, f = scale * factor;
-    map_chunk<T, G>(z, out, first, v.classes, tid, [&](float y, int64_t) { return none ? 0.f : unlisted_grad(y, ref2, f, a.c); });
+    const float x = a.aux[3 * rows + r];
+    const RowGradient o{a.aux[r], a.aux[rows + r], a.aux[2 * rows + r], a.tail ? x : (x == -INFINITY ? 0.f : 1.f), a.tail ? 0.f : x};
+    const bool none = o.lse == -INFINITY || w == 0.f;
+    const float ref2 = none ? 0.f : o.ref * LOG2E, f = none ? 0.f : scale * o.factor;
+    map_chunk<T, G, ONCE>(z, out, first, v.classes, tid, [&](float y, int64_t) { return none ? 0.f : unlisted_grad(y, ref2, f, a.c); });
     group_sync<G>();
-    if (!none) listed_grad<T, G>(a, out, list, first, CHUNK, lse, mass, norm, scale, tid);
+    if (!none) listed_grad<T, G>(a, out, list, first, CHUNK, o, scale, tid);
 }
 
-// Loss and gradient in one kernel, the row in the registers of G threads (HELD vectors each) between its one read and its gradient's
-// write.  A second read of a row of 256 KB would come from HBM: the rows in flight are larger than the caches.
-constexpr int HELD = 16;
-// the compiler may not carry what it unpacked from q past this point (two or four times the registers of q itself)
-__device__ __forceinline__ void keep_packed(uint4v (&q)[HELD]) {
-#pragma unroll
-    for (int h = 0; h < HELD; ++h) asm volatile("" : "+v"(q[h]));
-}
-template <typename T, int G, bool TAIL>
-__global__ __launch_bounds__(G < 256 ? 256 : G, 4) void distill_step_kernel(LogitsView v, int64_t rows, DistillArgs a, T* __restrict__ grad) {
+// Loss and gradient in one kernel: the row is read twice, the second time from cache, and its gradient written.  So that the second
+// read finds it there, G is chosen to leave few rows in flight: 2048 / G blocks on a CU.
+constexpr int STEP_U = 2;                                       // 64 registers: two blocks of 1024 threads on a CU
+template <typename T, int G, bool TAIL, int ONCE>
+__global__ __launch_bounds__(G < 256 ? 256 : G, 8) void distill_step_kernel(LogitsView v, int64_t rows, DistillArgs a, T* __restrict__ grad) {
     constexpr int BLOCK = G < 256 ? 256 : G, GROUPS = BLOCK / G, N = Vec<T>::N;
     extern __shared__ int dyn[];
     __shared__ Partial waves[BLOCK / 64];
-    __shared__ RowDistill shared_row;
+    __shared__ RowGradient shared_row[GROUPS];
     const int g = threadIdx.x / G, tid = threadIdx.x % G, lane = threadIdx.x & 63;
     const int64_t r = (int64_t)blockIdx.x * GROUPS + g;
     if (r >= rows) return;
-    const int n = (int)v.classes, nfull = n / N;
-    const int words = TAIL ? mark_words<T, G>(n) : 0;
+    const int n = (int)v.classes;
+    const int words = TAIL ? mark_words<T, G, STEP_U>(n) : 0;
     const ListLds list = list_lds(dyn + g * (3 * a.k + words), a.k);
     unsigned* bits = reinterpret_cast<unsigned*>(list.z + a.k);
     const RowPos p = row_pos(v, r);
     const T* z = static_cast<const T*>(v.p) + row_start(v, p);
     T* out = grad + r * v.classes;
-    const float w = a.weight ? a.weight[r] : 1.f;
-    uint4v q[HELD];                                             // beyond the row: -inf
-#pragma unroll
-    for (int h = 0; h < HELD; ++h) {
-        q[h] = raw_neg_inf<T>();
-        if (tid + h * G < nfull) q[h] = load_raw(z + (int64_t)(tid + h * G) * N);
-    }
-    const bool has_edge = nfull * N < n && nfull % G == tid;    // the last, partial vector
-    float edge[N];
-#pragma unroll
-    for (int j = 0; j < N; ++j) edge[j] = has_edge && nfull * N + j < n ? to_f32(z[nfull * N + j]) : -INFINITY;
     if (tid < 64) list_load(a, list_pos(v, p, r, a.k), z, v.classes, lane, list);
     group_sync<G>();
-    if (TAIL) mark_listed<T, G>(list.i, a.k, 0, n, bits, tid);
-    // (tail) the listed classes leave the registers: their logits and gradients come from the list
-    Online on;
-#pragma unroll
-    for (int h = 0; h < HELD; ++h) {
-        if (h * G >= nfull) continue;                           // of the whole group
-        if (TAIL) {
-            const unsigned b = (bits[h / UNROLL * G + tid] >> (h % UNROLL * 8)) & 0xFFu;
-            if (b) q[h] = raw_drop(q[h], b, (T*)nullptr);
-        }
-        float x[N];
-        unpack(q[h], x, (T*)nullptr);
-        on.m = fmaxf(on.m, max_of(x));
-    }
-    if (has_edge) {
-        if (TAIL) drop_listed(edge, (bits[nfull / (UNROLL * G) * G + tid] >> (nfull / G % UNROLL * 8)) & 0xFFu);
-        on.m = fmaxf(on.m, max_of(edge));
-    }
-    keep_packed(q);
-    const auto sums = [&](auto far_) {
-        constexpr bool FAR = decltype(far_)::value;             // some lane's maximum is -inf, or beyond BIG
-        const bool far = FAR && !(fabsf(on.m) <= BIG);
-        const float R = far ? 0.f : reference(on.m, a.c), sub = on.m == -INFINITY ? 0.f : on.m;
-        const auto term = [&](float f) { return exp2_hw(FAR && far ? (f - sub) * a.c : fmaf(f, a.c, -R)); };
-#pragma unroll
-        for (int h = 0; h < HELD; ++h) {
-            if (h * G >= nfull) continue;
-            float x[N];
-            unpack(q[h], x, (T*)nullptr);
-#pragma unroll
-            for (int j = 0; j < N; ++j) on.s += term(x[j]);
-        }
-        if (has_edge) {
-#pragma unroll
-            for (int j = 0; j < N; ++j) on.s += term(edge[j]);
-        }
-    };
-    if (__builtin_expect(__any(!(fabsf(on.m) <= BIG)), 0)) sums(std::true_type());
-    else sums(std::false_type());
-    keep_packed(q);
-    on = group_join<G>(on, a.c, waves);
-    RowDistill o;
+    if (TAIL) mark_listed<T, G, STEP_U>(list.i, a.k, 0, n, bits, tid);
+    const Online on = group_join<G>(distill_stream<T, G, TAIL, STEP_U, ONCE>(z, n, tid, bits, a.c), a.c, waves);
+    RowGradient o;
     if (tid < 64) {
-        o = distill_finish(a, list, on.m, on.s, lane);
-        if (lane == 0) a.loss[r] = w == 0.f ? 0.f : o.loss * w;
+        o = finish_row(a, list, on.m, on.s, r, rows, lane);
+        if (lane == 0) shared_row[g] = o;
     }
     if (G > 64) {
-        if (threadIdx.x == 0) shared_row = o;
         __syncthreads();
-        o = shared_row;
+        o = shared_row[g];
     }
-    const float scale = w * a.t;
-    const bool none = o.lse == -INFINITY || w == 0.f;
-    const float ref2 = none ? 0.f : o.ref * LOG2E, f = scale * o.factor;
+    const float scale = a.t * (a.weight ? a.weight[r] : 1.f);
+    const bool none = o.lse == -INFINITY || scale == 0.f;
+    const float ref2 = none ? 0.f : o.ref * LOG2E, f = none ? 0.f : scale * o.factor;
+    const auto put = [&](const float(&y)[N], int vec) {
+        float d[N];
 #pragma unroll
-    for (int h = 0; h < HELD; ++h) {
-        if (tid + h * G < nfull) {
-            float x[N];
-            unpack(q[h], x, (T*)nullptr);
+        for (int j = 0; j < N; ++j) d[j] = none ? 0.f : unlisted_grad(y[j], ref2, f, a.c);
+        if (vec < n / N) store_vec<ONCE != ONCE_NONE>(out + (int64_t)vec * N, d);
+        else if (vec * N < n) {
+            const int shift = edge_shift<T>(n, vec);
 #pragma unroll
-            for (int j = 0; j < N; ++j) x[j] = none ? 0.f : unlisted_grad(x[j], ref2, f, a.c);
-            store_vec(out + (int64_t)(tid + h * G) * N, x);
+            for (int j = 0; j < N; ++j)
+                if (j >= shift) out[n - N + j] = from_f32<T>(d[j]);
         }
-    }
-    if (has_edge) {
+    };
+    stream_row<T, G, STEP_U, ONCE>(
+        z, n, tid,
+        [&](const uint4v(&q)[STEP_U], int i) {
 #pragma unroll
-        for (int j = 0; j < N; ++j)
-            if (nfull * N + j < n) out[nfull * N + j] = from_f32<T>(none ? 0.f : unlisted_grad(edge[j], ref2, f, a.c));
-    }
+            for (int u = 0; u < STEP_U; ++u) {
+                float y[N];
+                unpack(q[u], y, (T*)nullptr);
+                put(y, i + u * G);
+            }
+        },
+        put);
     group_sync<G>();
-    if (!none) listed_grad<T, G>(a, out, list, 0, n, o.lse, o.mass, o.norm, scale, tid);
+    if (!none) listed_grad<T, G>(a, out, list, 0, n, o, scale, tid);
 }
 
 // ========================================================================================================================================
@@ -1238,6 +1300,17 @@ template <typename F> void by_bool(bool b, F&& f) {
 }
 }  // namespace
 
+// f(ONCE) for a kernel that reads (READS: and nothing of the call reads the rows again) and writes (WRITES) as much as the logits hold
+template <bool READS, bool WRITES, typename F> static void by_once(const LogitsView& v, int64_t rows, F&& f) {
+    const int64_t size = v.dtype == MICA_F32 ? 4 : 2, bytes = rows * v.classes * size;
+    const bool aligned = (((uintptr_t)v.p | (uintptr_t)(v.so * size) | (uintptr_t)(v.si * size)) & 15) == 0;
+    if constexpr (READS)
+        if (aligned && bytes > (int64_t)256 << 20) return f(std::integral_constant<int, ONCE_BOTH>());
+    if constexpr (WRITES)
+        if (bytes > (int64_t)64 << 20) return f(std::integral_constant<int, ONCE_STORE>());
+    f(std::integral_constant<int, ONCE_NONE>());
+}
+
 bool score_is_col(const LogitsView& v) { return v.classes <= SCORE_COL_MAX; }
 
 // Few long rows: cut so that about 512 blocks have work, no segment below 4096 classes; and no segment beyond what a block's bits take
@@ -1281,8 +1354,11 @@ void launch_score(const LogitsView& v, int64_t rows, const void* tokens, int tok
         const int64_t items = rows * s.n;
         by_bool(top > 0, [&](auto has_top) {
             constexpr bool TOP = decltype(has_top)::value;
-            if (wave_rows(v)) hipLaunchKernelGGL((score_row_kernel<T, 64, TOP>), dim3(blocks_of(items, 4)), dim3(256), 0, st, v, rows, o, s.n, s.len, part, part_top);
-            else hipLaunchKernelGGL((score_row_kernel<T, 256, TOP>), dim3((unsigned)items), dim3(256), 0, st, v, rows, o, s.n, s.len, part, part_top);
+            by_once<!TOP, false>(v, rows, [&](auto once) {      // the alternatives are read again
+                constexpr int ONCE = decltype(once)::value;
+                if (wave_rows(v)) hipLaunchKernelGGL((score_row_kernel<T, 64, TOP, ONCE>), dim3(blocks_of(items, 4)), dim3(256), 0, st, v, rows, o, s.n, s.len, part, part_top);
+                else hipLaunchKernelGGL((score_row_kernel<T, 256, TOP, ONCE>), dim3((unsigned)items), dim3(256), 0, st, v, rows, o, s.n, s.len, part, part_top);
+            });
             if (s.n > 1) hipLaunchKernelGGL((score_join_kernel<T, TOP>), dim3((unsigned)rows), dim3(TOP ? JOIN : 64), 0, st, v, o, s.n, part, part_top);
         });
     });
@@ -1302,18 +1378,22 @@ void launch_score_grad(const LogitsView& v, int64_t rows, const void* tokens, in
         }
         const int g = wave_rows(v) ? 64 : 256, chunk = g * UNROLL * vec_elems(v.dtype);
         const int chunks = (int)((v.classes + chunk - 1) / chunk);
-        if (g == 64) hipLaunchKernelGGL((score_grad_row_kernel<T, 64>), dim3(blocks_of(rows * chunks, 4)), dim3(256), 0, st, v, rows, o, chunks, out);
-        else hipLaunchKernelGGL((score_grad_row_kernel<T, 256>), dim3((unsigned)(rows * chunks)), dim3(256), 0, st, v, rows, o, chunks, out);
+        by_once<true, true>(v, rows, [&](auto once) {
+            constexpr int ONCE = decltype(once)::value;
+            if (g == 64) hipLaunchKernelGGL((score_grad_row_kernel<T, 64, ONCE>), dim3(blocks_of(rows * chunks, 4)), dim3(256), 0, st, v, rows, o, chunks, out);
+            else hipLaunchKernelGGL((score_grad_row_kernel<T, 256, ONCE>), dim3((unsigned)(rows * chunks)), dim3(256), 0, st, v, rows, o, chunks, out);
+        });
     });
 }
 
-// threads that hold a row in distill_step_kernel; 0: the row is too long, or rows are too few for a block each
+// Threads per row in distill_step_kernel; 0: rows are too few for a block each, or a block's bits do not cover them.  2048 / group rows
+// are in flight on each CU, and they have to fit the 256 MB of Infinity Cache: rows of 64 KB take 155 us at 256 threads (4096 of them)
+// and 204 at 1024, where the steps of a row are too short for so many waves; rows of 250 KB 534 at 512 and 509 at 1024.
 static int step_group(const LogitsView& v, int64_t rows) {
     if (score_segments(v, rows).n > 1) return 0;
-    const int64_t nvec = v.classes / vec_elems(v.dtype);
-    for (int g : {64, 256, 512, 1024})
-        if (nvec <= (int64_t)HELD * g) return g;
-    return 0;
+    if (wave_rows(v)) return 64;
+    const int64_t bytes = v.classes * (v.dtype == MICA_F32 ? 4 : 2);
+    return bytes <= 131072 ? 256 : bytes <= 196608 ? 512 : 1024;
 }
 
 int64_t distill_ws_bytes(const LogitsView& v, int64_t rows, bool step) {
@@ -1330,12 +1410,16 @@ static void distill_loss_rows(const LogitsView& v, int64_t rows, const DistillAr
         const int64_t items = rows * s.n;
         by_bool(a.tail, [&](auto tail) {
             constexpr bool TAIL = decltype(tail)::value;
-            if (wave_rows(v))
-                hipLaunchKernelGGL((distill_row_kernel<T, 64, TAIL>), dim3(blocks_of(items, 4)), dim3(256), 16u * (3 * a.k + (TAIL ? mark_words<T, 64>(s.len) : 0)), st, v,
-                                   rows, a, s.n, s.len, part);
-            else
-                hipLaunchKernelGGL((distill_row_kernel<T, 256, TAIL>), dim3((unsigned)items), dim3(256), 4u * (3 * a.k + (TAIL ? mark_words<T, 256>(s.len) : 0)), st, v,
-                                   rows, a, s.n, s.len, part);
+            by_once<true, false>(v, rows, [&](auto once) {
+                constexpr int ONCE = decltype(once)::value;
+                const auto lds = [&](int words, int groups) { return 4u * groups * (3 * a.k + (TAIL ? words : 0)); };
+                if (wave_rows(v))
+                    hipLaunchKernelGGL((distill_row_kernel<T, 64, TAIL, ONCE>), dim3(blocks_of(items, 4)), dim3(256), lds(mark_words<T, 64>(s.len), 4), st, v, rows, a, s.n,
+                                       s.len, part);
+                else
+                    hipLaunchKernelGGL((distill_row_kernel<T, 256, TAIL, ONCE>), dim3((unsigned)items), dim3(256), lds(mark_words<T, 256>(s.len), 1), st, v, rows, a, s.n,
+                                       s.len, part);
+            });
         });
         if (s.n > 1) hipLaunchKernelGGL((distill_join_kernel<T>), dim3((unsigned)rows), dim3(64), LIST_BYTES * a.k, st, v, rows, a, s.n, part);
     });
@@ -1346,8 +1430,11 @@ static void distill_grad_rows(const LogitsView& v, int64_t rows, const DistillAr
         T* out = static_cast<T*>(grad);
         const int g = wave_rows(v) ? 64 : 256, chunk = g * UNROLL * vec_elems(v.dtype);
         const int chunks = (int)((v.classes + chunk - 1) / chunk);
-        if (g == 64) hipLaunchKernelGGL((distill_grad_row_kernel<T, 64>), dim3(blocks_of(rows * chunks, 4)), dim3(256), 4 * LIST_BYTES * a.k, st, v, rows, a, chunks, out);
-        else hipLaunchKernelGGL((distill_grad_row_kernel<T, 256>), dim3((unsigned)(rows * chunks)), dim3(256), LIST_BYTES * a.k, st, v, rows, a, chunks, out);
+        by_once<true, true>(v, rows, [&](auto once) {
+            constexpr int ONCE = decltype(once)::value;
+            if (g == 64) hipLaunchKernelGGL((distill_grad_row_kernel<T, 64, ONCE>), dim3(blocks_of(rows * chunks, 4)), dim3(256), 4 * LIST_BYTES * a.k, st, v, rows, a, chunks, out);
+            else hipLaunchKernelGGL((distill_grad_row_kernel<T, 256, ONCE>), dim3((unsigned)(rows * chunks)), dim3(256), LIST_BYTES * a.k, st, v, rows, a, chunks, out);
+        });
     });
 }
 template <bool LOSS, bool GRAD> static void distill_col(const LogitsView& v, int64_t rows, const DistillArgs& a, void* grad, hipStream_t st) {
@@ -1408,14 +1495,18 @@ void launch_distill_step(const LogitsView& v, int64_t rows, const DistillList& d
         const int n = (int)v.classes;
         by_bool(a.tail, [&](auto tail) {
             constexpr bool TAIL = decltype(tail)::value;
-            if (group == 64)
-                hipLaunchKernelGGL((distill_step_kernel<T, 64, TAIL>), dim3(blocks_of(rows, 4)), dim3(256), 16u * (3 * a.k + (TAIL ? mark_words<T, 64>(n) : 0)), st, v, rows, a, out);
-            else if (group == 256)
-                hipLaunchKernelGGL((distill_step_kernel<T, 256, TAIL>), dim3((unsigned)rows), dim3(256), 4u * (3 * a.k + (TAIL ? mark_words<T, 256>(n) : 0)), st, v, rows, a, out);
-            else if (group == 512)
-                hipLaunchKernelGGL((distill_step_kernel<T, 512, TAIL>), dim3((unsigned)rows), dim3(512), 4u * (3 * a.k + (TAIL ? mark_words<T, 512>(n) : 0)), st, v, rows, a, out);
-            else
-                hipLaunchKernelGGL((distill_step_kernel<T, 1024, TAIL>), dim3((unsigned)rows), dim3(1024), 4u * (3 * a.k + (TAIL ? mark_words<T, 1024>(n) : 0)), st, v, rows, a, out);
+            by_once<false, true>(v, rows, [&](auto once) {      // the row is read again
+                constexpr int ONCE = decltype(once)::value;
+                const auto lds = [&](int words, int groups) { return 4u * groups * (3 * a.k + (TAIL ? words : 0)); };
+                if (group == 64)
+                    hipLaunchKernelGGL((distill_step_kernel<T, 64, TAIL, ONCE>), dim3(blocks_of(rows, 4)), dim3(256), lds(mark_words<T, 64, STEP_U>(n), 4), st, v, rows, a, out);
+                else if (group == 256)
+                    hipLaunchKernelGGL((distill_step_kernel<T, 256, TAIL, ONCE>), dim3((unsigned)rows), dim3(256), lds(mark_words<T, 256, STEP_U>(n), 1), st, v, rows, a, out);
+                else if (group == 512)
+                    hipLaunchKernelGGL((distill_step_kernel<T, 512, TAIL, ONCE>), dim3((unsigned)rows), dim3(512), lds(mark_words<T, 512, STEP_U>(n), 1), st, v, rows, a, out);
+                else
+                    hipLaunchKernelGGL((distill_step_kernel<T, 1024, TAIL, ONCE>), dim3((unsigned)rows), dim3(1024), lds(mark_words<T, 1024, STEP_U>(n), 1), st, v, rows, a, out);
+            });
         });
     });
 }
