@@ -414,11 +414,11 @@ struct TopNote {
         }
     }
 };
-template <typename T, int G> __device__ __forceinline__ int rounds_per_part(int n) {
-    const int rounds = n / Vec<T>::N / (UNROLL * G);
+template <typename T, int G, int U> __device__ __forceinline__ int rounds_per_part(int n) {
+    const int rounds = n / Vec<T>::N / (U * G);
     return rounds < PARTS ? 1 : rounds / PARTS;
 }
-template <typename T, int G>
+template <typename T, int G, int U>
 __device__ __forceinline__ u64 group_top(const T* __restrict__ z, int n, unsigned index0, int k, const TopNote& note, TopScratch* sc, int* owners,
                                          TopShared* sh) {
     constexpr int N = Vec<T>::N, NW = G / 64;
@@ -426,19 +426,33 @@ __device__ __forceinline__ u64 group_top(const T* __restrict__ z, int n, unsigne
     u64 mine = note.key[0];
 #pragma unroll
     for (int i = 1; i < PARTS; ++i) mine = note.key[i] > mine ? note.key[i] : mine;
-    u64 bound = lane_key(sort64<true>(mine, lane), (k + NW - 1) / NW - 1);
+    // waves whose threads all have a class share the K; with none, everything passes
+    const int whole = NW == 1 ? 1 : (n / N / 64 < NW ? n / N / 64 : NW);
+    const int nth = whole == 0 ? 0 : (k + whole - 1) / whole;
+    u64 bound = 0;
+    if (nth > 4) bound = lane_key(sort64<true>(mine, lane), nth - 1);
+    else {                                                      // a maximum costs a fifth of a sort
+        u64 left = mine;
+        for (int i = 0; i < nth; ++i) {
+            bound = wave_all(left, [](u64 a, u64 b) { return a > b ? a : b; });
+            left = left == bound ? 0 : left;
+        }
+        bound = lane_key(bound, 0);
+    }
     int count;
     if (NW > 1) {
         if (lane == 0) sh->bound[w] = bound;
         if (threadIdx.x == 0) sh->owners_n = sh->passed = 0;
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < NW; ++i) bound = sh->bound[i] < bound ? sh->bound[i] : bound;
+        for (int i = 0; i < NW; ++i)
+            if (i < whole) bound = i == 0 || sh->bound[i] < bound ? sh->bound[i] : bound;
+        bound = lane_key(bound, 0);
 #pragma unroll
         for (int i = 0; i < PARTS; ++i)                         // the order of the owners does not change the result
             if (note.key[i] != 0 && note.key[i] >= bound) owners[atomicAdd(&sh->owners_n, 1)] = i * G + tid;
         __syncthreads();
-        count = sh->owners_n;
+        count = __builtin_amdgcn_readfirstlane(sh->owners_n);       // scalar: what follows branches for the whole block
     } else {
         count = 0;
 #pragma unroll
@@ -450,18 +464,19 @@ __device__ __forceinline__ u64 group_top(const T* __restrict__ z, int n, unsigne
         }
         wave_sync();
     }
-    const int nvec = (n + N - 1) / N, rounds = nvec / (UNROLL * G) + 1, per_part = rounds_per_part<T, G>(n);
+    const float bound_value = key_value((unsigned)(bound >> 32));       // (of 0: NaN, below which nothing is)
+    const int nvec = (n + N - 1) / N, rounds = nvec / (U * G) + 1, per_part = rounds_per_part<T, G, U>(n);
     // the longest stretch, in vectors of one thread: the last one
-    const int per = (rounds - (PARTS - 1) * per_part > per_part ? rounds - (PARTS - 1) * per_part : per_part) * UNROLL;
+    const int per = (rounds - (PARTS - 1) * per_part > per_part ? rounds - (PARTS - 1) * per_part : per_part) * U;
     const int total = count * per;
-    // take(passes, key), by whole waves, for every class the owners hold
+    // take(passes, key), by whole waves, for the classes the owners hold, at least those that pass
     const auto scan = [&](auto&& take) {
         for (int p0 = 0; p0 < total; p0 += G) {
             const int p = p0 + tid;
             int vec = nvec;
             if (p < total) {
                 const int own = owners[p % count], part = own / G, i = p / count;       // the i-th vector of the stretch
-                if (part == PARTS - 1 || i < per_part * UNROLL) vec = own % G + (part * per_part * UNROLL + i) * G;
+                if (part == PARTS - 1 || i < per_part * U) vec = own % G + (part * per_part * U + i) * G;
                 if (vec > nvec) vec = nvec;
             }
             const int shift = edge_shift<T>(n, vec);
@@ -469,6 +484,7 @@ __device__ __forceinline__ u64 group_top(const T* __restrict__ z, int n, unsigne
             unpack(load_vec(z, n, vec), v, (T*)nullptr);
 #pragma unroll
             for (int j = 0; j < N; ++j) {
+                if (!__any(!(v[j] < bound_value))) continue;    // NaN counts as -inf
                 const int at = vec * N + j - shift;
                 const unsigned o = order_key(v[j]);
                 take(vec < nvec && j >= shift && make_key(o, (unsigned)(vec * N)) >= bound, make_key(o, (unsigned)at));
@@ -485,7 +501,7 @@ __device__ __forceinline__ u64 group_top(const T* __restrict__ z, int n, unsigne
             }
         });
         __syncthreads();
-        const int passed = sh->passed;
+        const int passed = __builtin_amdgcn_readfirstlane(sh->passed);
         few = passed <= 64;
         if (few) {
             if (w == 0) list = sort64<true>(lane < passed ? sc[0].buf[lane] : 0, lane);
@@ -573,7 +589,7 @@ __device__ __forceinline__ void write_top(const ScoreOut& o, const LogitsView& v
 template <typename T, int G, bool TOP, int ONCE>
 __global__ __launch_bounds__(256) void score_row_kernel(LogitsView v, int64_t rows, ScoreOut o, int segments, int seg_len, Partial* __restrict__ part,
                                                         u64* __restrict__ part_top) {
-    constexpr int N = Vec<T>::N, NW = G / 64, GROUPS = 256 / G;
+    constexpr int N = Vec<T>::N, NW = G / 64, GROUPS = 256 / G, U = TOP ? 2 : UNROLL;
     __shared__ Partial waves[4];
     __shared__ TopScratch top_sc[TOP ? 4 : 1];
     __shared__ int owners[TOP ? 256 * PARTS : 1];
@@ -589,14 +605,14 @@ __global__ __launch_bounds__(256) void score_row_kernel(LogitsView v, int64_t ro
     const int n = (int)(v.classes - first < seg_len ? v.classes - first : seg_len);
     Online on;
     TopNote note;
-    const int per_part = rounds_per_part<T, G>(n);
+    const int per_part = rounds_per_part<T, G, U>(n);
     if (TOP) note.start(per_part);
-    stream_row<T, G, UNROLL, ONCE>(
+    stream_row<T, G, U, ONCE>(
         z + first, n, tid,
-        [&](const uint4v(&q)[UNROLL], int i) {
-            float f[UNROLL * N], vm = -INFINITY;
+        [&](const uint4v(&q)[U], int i) {
+            float f[U * N], vm = -INFINITY;
 #pragma unroll
-            for (int u = 0; u < UNROLL; ++u) {
+            for (int u = 0; u < U; ++u) {
                 float x[N];
                 unpack(q[u], x, (T*)nullptr);
                 const float mu = max_of(x);
@@ -606,7 +622,7 @@ __global__ __launch_bounds__(256) void score_row_kernel(LogitsView v, int64_t ro
                 for (int j = 0; j < N; ++j) f[u * N + j] = x[j];
             }
             if (TOP) note.round_done(per_part);
-            on.add<UNROLL * N, true>(f, vm, o.c);
+            on.add<U * N, true>(f, vm, o.c);
         },
         [&](const float(&f)[N], int vec) {
             const float vm = max_of(f);
@@ -617,7 +633,7 @@ __global__ __launch_bounds__(256) void score_row_kernel(LogitsView v, int64_t ro
     u64 key = 0;
     if (TOP) {
         note.close();
-        key = group_top<T, G>(z + first, n, (unsigned)first, o.top, note, NW == 1 ? &top_sc[g] : top_sc, &owners[g * G * PARTS], &top_sh);
+        key = group_top<T, G, U>(z + first, n, (unsigned)first, o.top, note, NW == 1 ? &top_sc[g] : top_sc, &owners[g * G * PARTS], &top_sh);
     }
     if (segments == 1) {
         if (tid < 64) {
@@ -1325,7 +1341,7 @@ SegPlan score_segments(const LogitsView& v, int64_t rows) {
     n = std::max<int64_t>(n, (v.classes + longest - 1) / longest);
     if (n <= 1) return s;
     int64_t len = (v.classes + n - 1) / n;
-    len = (len + 511) / 512 * 512;                          // 16-byte vectors of a segment begin where the row's do
+    len = (len + 63) / 64 * 64;                             // 16-byte vectors of a segment begin where the row's do; the last is not much shorter
     s.len = (int)len;
     s.n = (int)((v.classes + len - 1) / len);
     return s;

@@ -19,6 +19,10 @@ def _ptr(t):
     return None if t is None else C.c_void_p(t.data_ptr())
 
 
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
 def _f32c(t: torch.Tensor, name: str) -> torch.Tensor:
     if t.dtype != torch.float32 or not t.is_cuda:
         raise MicaHipError(f"{name}: expected a float32 CUDA(HIP) tensor, got {t.dtype} on {t.device}")
@@ -71,6 +75,11 @@ class Engine:
     def _stream(self):
         """torch's current stream of THIS engine's device (the C side does hipSetDevice(ctx->device))."""
         return C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
+
+    def _raw_stream(self):
+        """_stream() as an integer, without the Stream object where torch offers the handle itself (4 us of a call of 15)."""
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        return raw(self.device.index) if raw else torch.cuda.current_stream(self.device).cuda_stream
 
     def _check(self, r, what):
         if r != 0:
@@ -374,7 +383,8 @@ class Engine:
         return dis, mat
 
     # -- scoring of class distributions, distillation from top alternatives (mica_amd/scoring.py: the differentiable forms) --------
-    def _logits(self, logits, dim, name="logits"):
+    def logits_view(self, logits, dim, name="logits"):
+        """The library's view of a logits tensor (scoring.LogitsLayout); the calls below take one that was made for the same tensor."""
         if not isinstance(logits, torch.Tensor) or logits.device != self.device:
             raise MicaHipError(f"{name}: expected a tensor on {self.device}, got {getattr(logits, 'device', type(logits))}")
         return scoring.LogitsLayout(logits, dim)
@@ -385,108 +395,123 @@ class Engine:
             raise MicaHipError(f"workspace query refused ({nbytes})")
         return torch.empty((nbytes,), dtype=torch.uint8, device=self.device) if nbytes else None
 
-    def _f32_rows(self, shape):
-        return torch.empty(shape, dtype=torch.float32, device=self.device)
-
     def token_logprobs(self, logits: torch.Tensor, tokens: torch.Tensor | None = None, top: int = 0, dim: int = -1, temperature: float = 1.0,
-                       ignore_index: int = -100):
+                       ignore_index: int = -100, view=None):
         """Scores of the distributions softmax(logits / temperature) along `dim` -> scoring.TokenScores:
         logprob (of `tokens`, integers of the logits' shape without `dim`; ignore_index: 0, any other value outside [0, classes): NaN),
         entropy and lse (log sum exp), all float32; top_logprob float32 / top_index int32, the `top` (<= 64) most probable classes in
         order, ties to the lowest class.  Logits float32, bfloat16 or float16 of any strides.  A row whose classes are all -inf: log
         probabilities -inf, entropy 0.  Asynchronous; the results have no autograd history (scoring.token_logprobs has)."""
-        v = self._logits(logits, dim)
+        v = self.logits_view(logits, dim) if view is None else view
         temperature = scoring.check_temperature(temperature)
         top = int(top)
         if not 0 <= top <= min(scoring.MAX_TOP, v.classes):
             raise MicaHipError(f"top must be in [0, {min(scoring.MAX_TOP, v.classes)}], got {top}")
+        dev, shape = self.device, v.rows_shape
         logprob = topv = topi = None
         if tokens is not None:
-            tokens = scoring.check_ints(tokens, "tokens", v.rows_shape, self.device).contiguous()
-            logprob = self._f32_rows(v.rows_shape)
-        entropy, lse = self._f32_rows(v.rows_shape), self._f32_rows(v.rows_shape)
+            tokens = scoring.check_ints(tokens, "tokens", shape, dev).contiguous()
+            logprob = torch.empty(shape, dtype=torch.float32, device=dev)
+        entropy = torch.empty(shape, dtype=torch.float32, device=dev)
+        lse = torch.empty(shape, dtype=torch.float32, device=dev)
         if top:
-            topv = self._f32_rows(v.with_axis(top))
-            topi = torch.empty(v.with_axis(top), dtype=torch.int32, device=self.device)
+            lists = v.with_axis(top)
+            topv = torch.empty(lists, dtype=torch.float32, device=dev)
+            topi = torch.empty(lists, dtype=torch.int32, device=dev)
         if v.rows:
-            ws = self._workspace(self.lib.mica_token_logprobs_ws(C.byref(v.desc), top))
-            self._check(self.lib.mica_token_logprobs(
-                self._h, C.byref(v.desc), _ptr(tokens), 0 if tokens is None else tokens.element_size(), int(ignore_index), temperature, top,
-                _ptr(logprob), _ptr(entropy), _ptr(lse), _ptr(topv), _ptr(topi), _ptr(ws), 0 if ws is None else ws.numel(), self._stream()),
-                "mica_token_logprobs")
-        return scoring.TokenScores(logprob, entropy, lse, None if topv is None else v.give(topv), None if topi is None else v.give(topi))
+            z = C.byref(v.desc)
+            nws = self.lib.mica_token_logprobs_ws(z, top)
+            ws = self._workspace(nws)
+            r = self.lib.mica_token_logprobs(self._h, z, _addr(tokens), tokens.element_size() if tokens is not None else 0, int(ignore_index), temperature,
+                                             top, _addr(logprob), entropy.data_ptr(), lse.data_ptr(), _addr(topv), _addr(topi), _addr(ws), nws,
+                                             self._raw_stream())
+            self._check(r, "mica_token_logprobs")
+        if v.moved and top:
+            topv, topi = v.give(topv), v.give(topi)
+        return scoring.TokenScores(logprob, entropy, lse, topv, topi)
 
     def token_logprobs_backward(self, logits, tokens, lse, entropy, g_logprob=None, g_entropy=None, g_lse=None, dim: int = -1,
-                                temperature: float = 1.0, ignore_index: int = -100) -> torch.Tensor:
+                                temperature: float = 1.0, ignore_index: int = -100, view=None) -> torch.Tensor:
         """Gradient, in the logits' type and shape, of (g_logprob logprob + g_entropy entropy + g_lse lse).sum(); lse and entropy are
         token_logprobs' results for the same logits and temperature; each upstream gradient may be None."""
-        v = self._logits(logits, dim)
+        v = self.logits_view(logits, dim) if view is None else view
         temperature = scoring.check_temperature(temperature)
-        rows = []
-        for t, name in ((lse, "lse"), (entropy, "entropy"), (g_logprob, "g_logprob"), (g_entropy, "g_entropy"), (g_lse, "g_lse")):
-            if t is None and name.startswith("g_"):
-                rows.append(None)
-            else:
-                rows.append(scoring.check_floats(t, name, v.rows_shape, self.device).contiguous())
+        dev, shape = self.device, v.rows_shape
+        lse = scoring.check_floats(lse, "lse", shape, dev).contiguous()
+        entropy = scoring.check_floats(entropy, "entropy", shape, dev).contiguous()
+        if g_entropy is not None:
+            g_entropy = scoring.check_floats(g_entropy, "g_entropy", shape, dev).contiguous()
+        if g_lse is not None:
+            g_lse = scoring.check_floats(g_lse, "g_lse", shape, dev).contiguous()
         if g_logprob is not None:
-            tokens = scoring.check_ints(tokens, "tokens", v.rows_shape, self.device).contiguous()
+            g_logprob = scoring.check_floats(g_logprob, "g_logprob", shape, dev).contiguous()
+            tokens = scoring.check_ints(tokens, "tokens", shape, dev).contiguous()
         else:
             tokens = None
-        grad = torch.empty(v.with_axis(v.classes), dtype=logits.dtype, device=self.device)
+        grad = torch.empty(v.with_axis(v.classes), dtype=v.dtype, device=dev)
         if v.rows:
-            self._check(self.lib.mica_token_logprobs_backward(
-                self._h, C.byref(v.desc), _ptr(tokens), 0 if tokens is None else tokens.element_size(), int(ignore_index), temperature,
-                *[_ptr(t) for t in rows], _ptr(grad), self._stream()), "mica_token_logprobs_backward")
+            r = self.lib.mica_token_logprobs_backward(self._h, C.byref(v.desc), _addr(tokens), tokens.element_size() if tokens is not None else 0,
+                                                      int(ignore_index), temperature, lse.data_ptr(), entropy.data_ptr(), _addr(g_logprob),
+                                                      _addr(g_entropy), _addr(g_lse), grad.data_ptr(), self._raw_stream())
+            self._check(r, "mica_token_logprobs_backward")
         return v.give(grad)
 
     def distill_loss(self, student: torch.Tensor, teacher_index: torch.Tensor, teacher_logprob: torch.Tensor, dim: int = -1,
-                     temperature: float = 1.0, tail: bool = False):
+                     temperature: float = 1.0, tail: bool = False, view=None):
         """Kullback-Leibler divergence, times temperature^2, of softmax(student / temperature) from a teacher known by its K (<= 256)
         top alternatives per row -> (loss float32, rows; aux for distill_backward).
         teacher_index (int32 / int64, negative = unused entry) and teacher_logprob (log probabilities at the same temperature, e.g.
         token_logprobs(teacher, top=K, temperature=T)) have K at axis `dim`.  tail=False: the list is renormalised over its K entries;
         tail=True: all classes not listed share the teacher's remaining mass 1 - sum p as one alternative.  A row without used entries
         has loss 0; a student row of -inf only: loss +inf, gradient 0; an index >= classes: NaN."""
-        v = self._logits(student, dim, "student")
+        v = self.logits_view(student, dim, "student") if view is None else view
         temperature = scoring.check_temperature(temperature)
         lst, keep = scoring.top_list(v, teacher_index, teacher_logprob, tail, self.device)
-        loss = self._f32_rows(v.rows_shape)
-        aux = self._f32_rows((4, v.rows) if v.classes > scoring.COL_MAX else (0,))
+        loss = torch.empty(v.rows_shape, dtype=torch.float32, device=self.device)
+        aux = torch.empty((4, v.rows) if v.classes > scoring.COL_MAX else (0,), dtype=torch.float32, device=self.device)
         if v.rows:
-            ws = self._workspace(self.lib.mica_distill_ws(C.byref(v.desc), 0))
-            self._check(self.lib.mica_distill_loss(self._h, C.byref(v.desc), C.byref(lst), temperature, _ptr(loss), _ptr(aux) if aux.numel() else None,
-                                                   _ptr(ws), 0 if ws is None else ws.numel(), self._stream()), "mica_distill_loss")
+            z = C.byref(v.desc)
+            nws = self.lib.mica_distill_ws(z, 0)
+            ws = self._workspace(nws)
+            r = self.lib.mica_distill_loss(self._h, z, C.byref(lst), temperature, loss.data_ptr(), aux.data_ptr() or None, _addr(ws), nws,
+                                           self._raw_stream())
+            self._check(r, "mica_distill_loss")
         del keep
         return loss, aux
 
-    def distill_backward(self, student, teacher_index, teacher_logprob, aux, g_loss, dim: int = -1, temperature: float = 1.0, tail: bool = False):
+    def distill_backward(self, student, teacher_index, teacher_logprob, aux, g_loss, dim: int = -1, temperature: float = 1.0, tail: bool = False,
+                         view=None):
         """Gradient, in the student's type and shape, of (g_loss * loss).sum(); aux: distill_loss' second result for the same arguments."""
-        v = self._logits(student, dim, "student")
+        v = self.logits_view(student, dim, "student") if view is None else view
         temperature = scoring.check_temperature(temperature)
         lst, keep = scoring.top_list(v, teacher_index, teacher_logprob, tail, self.device)
         aux = scoring.check_floats(aux, "aux", (4, v.rows) if v.classes > scoring.COL_MAX else (0,), self.device).contiguous()
         g_loss = scoring.check_floats(g_loss, "g_loss", v.rows_shape, self.device).contiguous()
-        grad = torch.empty(v.with_axis(v.classes), dtype=student.dtype, device=self.device)
+        grad = torch.empty(v.with_axis(v.classes), dtype=v.dtype, device=self.device)
         if v.rows:
-            self._check(self.lib.mica_distill_backward(self._h, C.byref(v.desc), C.byref(lst), temperature, _ptr(aux) if aux.numel() else None,
-                                                       _ptr(g_loss), _ptr(grad), self._stream()), "mica_distill_backward")
+            r = self.lib.mica_distill_backward(self._h, C.byref(v.desc), C.byref(lst), temperature, aux.data_ptr() or None, g_loss.data_ptr(),
+                                               grad.data_ptr(), self._raw_stream())
+            self._check(r, "mica_distill_backward")
         del keep
         return v.give(grad)
 
     def distill_step(self, student, teacher_index, teacher_logprob, dim: int = -1, temperature: float = 1.0, tail: bool = False, weight=None):
         """The training step's form: (weight * loss, gradient of its sum with respect to the student's logits) in one call.  weight
         float32, one per row (None: 1); rows of weight 0 give loss 0 and gradient 0 whatever they hold."""
-        v = self._logits(student, dim, "student")
+        v = self.logits_view(student, dim, "student")
         temperature = scoring.check_temperature(temperature)
         lst, keep = scoring.top_list(v, teacher_index, teacher_logprob, tail, self.device)
         if weight is not None:
             weight = scoring.check_floats(weight, "weight", v.rows_shape, self.device).contiguous()
-        loss = self._f32_rows(v.rows_shape)
-        grad = torch.empty(v.with_axis(v.classes), dtype=student.dtype, device=self.device)
+        loss = torch.empty(v.rows_shape, dtype=torch.float32, device=self.device)
+        grad = torch.empty(v.with_axis(v.classes), dtype=v.dtype, device=self.device)
         if v.rows:
-            ws = self._workspace(self.lib.mica_distill_ws(C.byref(v.desc), 1))
-            self._check(self.lib.mica_distill_step(self._h, C.byref(v.desc), C.byref(lst), temperature, _ptr(weight), _ptr(loss), _ptr(grad), _ptr(ws),
-                                                   0 if ws is None else ws.numel(), self._stream()), "mica_distill_step")
+            z = C.byref(v.desc)
+            nws = self.lib.mica_distill_ws(z, 1)
+            ws = self._workspace(nws)
+            r = self.lib.mica_distill_step(self._h, z, C.byref(lst), temperature, _addr(weight), loss.data_ptr(), grad.data_ptr(), _addr(ws), nws,
+                                           self._raw_stream())
+            self._check(r, "mica_distill_step")
         del keep
         return loss, v.give(grad)
 

@@ -12,6 +12,7 @@ sure the network is, and what the runners-up are.  A smaller network is then tra
 float32, bfloat16 or float16 logits: the last one of a language model's [B, S, C], axis 1 of a head's NCDHW logits, or a slice of either."""
 from __future__ import annotations
 
+import math
 import typing
 
 import torch
@@ -22,6 +23,7 @@ from ._cabi import MicaHipError
 COL_MAX = 64                # up to so many classes are read at any stride (kernels_score.hip)
 MAX_TOP = 64                # alternatives per row
 MAX_LIST = 256              # entries of a teacher's list
+INTS = (torch.int32, torch.int64)
 DTYPES = {torch.float32: _cabi.MICA_F32, torch.bfloat16: _cabi.MICA_BF16, torch.float16: _cabi.MICA_F16}
 
 
@@ -52,38 +54,41 @@ class LogitsLayout:
     """How a logits tensor is handed to the library: the view (`desc`), the tensor it points into (`base`: the logits themselves, or a
     copy where no view fits), and the shapes of what comes back.  `moved`: the copy has the class axis last, results are laid out like
     it and returned as views with the axis where the caller has it."""
+    __slots__ = ("dim", "shape", "classes", "rows_shape", "rows", "base", "moved", "class_last", "desc", "dtype")
 
     def __init__(self, logits: torch.Tensor, dim: int):
-        if not isinstance(logits, torch.Tensor) or logits.dtype not in DTYPES:
+        dtype = DTYPES.get(logits.dtype) if isinstance(logits, torch.Tensor) else None
+        if dtype is None:
             raise MicaHipError(f"logits: expected a float32, bfloat16 or float16 tensor, got {getattr(logits, 'dtype', type(logits))}")
-        if logits.dim() < 1 or not -logits.dim() <= dim < logits.dim():
-            raise MicaHipError(f"dim {dim} is no axis of logits of shape {tuple(logits.shape)}")
-        self.dim = dim % logits.dim()
-        self.shape = tuple(logits.shape)
-        self.classes = self.shape[self.dim]
-        self.rows_shape = self.shape[:self.dim] + self.shape[self.dim + 1:]
-        self.rows = 1
-        for n in self.rows_shape:
-            self.rows *= n
-        if not 1 <= self.classes <= 1 << 28:
-            raise MicaHipError(f"logits: 1 to 2^28 classes expected along axis {self.dim}, got {self.classes}")
-        if self.rows >= 1 << 31:
-            raise MicaHipError(f"logits: fewer than 2^31 rows expected, got {self.rows}")
+        shape = tuple(logits.shape)
+        if not shape or not -len(shape) <= dim < len(shape):
+            raise MicaHipError(f"dim {dim} is no axis of logits of shape {shape}")
+        self.dim = dim = dim % len(shape)
+        self.shape, self.dtype = shape, logits.dtype
+        self.classes = classes = shape[dim]
+        self.rows_shape = rows_shape = shape[:dim] + shape[dim + 1:]
+        self.rows = rows = math.prod(rows_shape)
+        if not 1 <= classes <= 1 << 28:
+            raise MicaHipError(f"logits: 1 to 2^28 classes expected along axis {dim}, got {classes}")
+        if rows >= 1 << 31:
+            raise MicaHipError(f"logits: fewer than 2^31 rows expected, got {rows}")
         self.base, self.moved = logits, False
-        view = self._view(logits, self.dim)
-        if view is None:
-            if self.classes > COL_MAX and self.dim != len(self.shape) - 1:
-                self.base, self.moved = logits.movedim(self.dim, -1).contiguous(), True
-                view = self._view(self.base, len(self.shape) - 1)
-            else:
-                self.base = logits.contiguous()
-                view = self._view(self.base, self.dim)
-        outer, inner, class_last, sc = view
-        self.class_last = class_last
-        self.desc = _cabi.MicaLogits(self.base.data_ptr(), DTYPES[logits.dtype], int(class_last), outer[0], inner[0], self.classes, outer[1],
-                                     inner[1], sc)
+        if dim == len(shape) - 1 and logits.is_contiguous():
+            outer, inner, self.class_last, sc = (1, 0), (rows, classes if rows > 1 else 0), True, 1
+        else:
+            view = self._view(logits, dim)
+            if view is None:
+                if classes > COL_MAX and dim != len(shape) - 1:
+                    self.base, self.moved = logits.movedim(dim, -1).contiguous(), True
+                    view = self._view(self.base, len(shape) - 1)
+                else:
+                    self.base = logits.contiguous()
+                    view = self._view(self.base, dim)
+            outer, inner, self.class_last, sc = view
+        self.desc = _cabi.MicaLogits(self.base.data_ptr(), dtype, self.class_last, outer[0], inner[0], classes, outer[1], inner[1], sc)
 
-    def _view(self, t, dim):
+    @staticmethod
+    def _view(t, dim):
         """-> ((outer, stride), (inner, stride), class_last, class stride), or None where the library has no view of t."""
         n, s = t.shape, t.stride()
         before, after = _collapse(n[:dim], s[:dim]), _collapse(n[dim + 1:], s[dim + 1:])
@@ -118,14 +123,14 @@ def check_temperature(t):
 
 
 def check_ints(t, name, shape, device):
-    if not isinstance(t, torch.Tensor) or t.dtype not in (torch.int32, torch.int64) or t.device != device or tuple(t.shape) != tuple(shape):
+    if not isinstance(t, torch.Tensor) or t.dtype not in INTS or t.shape != shape or t.device != device:
         got = f"{t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else type(t)
         raise MicaHipError(f"{name}: expected an int32 or int64 tensor of shape {tuple(shape)} on {device}, got {got}")
     return t
 
 
 def check_floats(t, name, shape, device, dtypes=(torch.float32,)):
-    if not isinstance(t, torch.Tensor) or t.dtype not in dtypes or t.device != device or tuple(t.shape) != tuple(shape):
+    if not isinstance(t, torch.Tensor) or t.dtype not in dtypes or t.shape != shape or t.device != device:
         got = f"{t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else type(t)
         raise MicaHipError(f"{name}: expected a {' / '.join(str(d) for d in dtypes)} tensor of shape {tuple(shape)} on {device}, got {got}")
     return t
@@ -140,7 +145,7 @@ def top_list(layout: LogitsLayout, index, value, tail, device):
         raise MicaHipError(f"teacher_index: 1 to {MAX_LIST} entries per row expected, got {k}")
     shape = layout.shape[:layout.dim] + (k,) + layout.shape[layout.dim + 1:]
     check_ints(index, "teacher_index", shape, device)
-    check_floats(value, "teacher_logprob", shape, device, tuple(DTYPES))
+    check_floats(value, "teacher_logprob", shape, device, DTYPES)
     index, value = layout.take(index), layout.take(value)
     return _cabi.MicaTopList(index.data_ptr(), value.data_ptr(), index.element_size(), DTYPES[value.dtype], k, int(bool(tail))), (index, value)
 
@@ -148,10 +153,13 @@ def top_list(layout: LogitsLayout, index, value, tail, device):
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, engine, tokens, top, dim, temperature, ignore_index):
-        r = engine.token_logprobs(logits, tokens, top, dim, temperature, ignore_index)
-        ctx.engine, ctx.args, ctx.has_tokens = engine, (dim, temperature, ignore_index), tokens is not None
-        ctx.save_for_backward(logits, r.lse, r.entropy, *([tokens] if tokens is not None else []))
-        ctx.mark_non_differentiable(*[t for t in (r.top_logprob, r.top_index) if t is not None])
+        view = engine.logits_view(logits, dim)
+        r = engine.token_logprobs(logits, tokens, top, dim, temperature, ignore_index, view)
+        ctx.call = engine, view, temperature, ignore_index, dim
+        # through save_for_backward, also what the view points into: torch refuses a backward pass over logits that were written since
+        ctx.save_for_backward(logits, r.lse, r.entropy, tokens)
+        if r.top_index is not None:
+            ctx.mark_non_differentiable(r.top_logprob, r.top_index)
         ctx.set_materialize_grads(False)
         return tuple(r)
 
@@ -160,9 +168,10 @@ class _TokenLogprobs(torch.autograd.Function):
     def backward(ctx, g_logprob, g_entropy, g_lse, *_):
         if g_logprob is None and g_entropy is None and g_lse is None:
             return (None,) * 7
-        logits, lse, entropy, *tokens = ctx.saved_tensors
-        grad = ctx.engine.token_logprobs_backward(logits, tokens[0] if ctx.has_tokens else None, lse, entropy, g_logprob, g_entropy, g_lse, *ctx.args)
-        return (grad,) + (None,) * 6
+        logits, lse, entropy, tokens = ctx.saved_tensors
+        engine, view, temperature, ignore_index, dim = ctx.call
+        return (engine.token_logprobs_backward(logits, tokens, lse, entropy, g_logprob, g_entropy, g_lse, dim, temperature, ignore_index, view),
+                None, None, None, None, None, None)
 
 
 def token_logprobs(engine, logits, tokens=None, top: int = 0, dim: int = -1, temperature: float = 1.0, ignore_index: int = -100) -> TokenScores:
@@ -173,8 +182,9 @@ def token_logprobs(engine, logits, tokens=None, top: int = 0, dim: int = -1, tem
 class _DistillLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, student, engine, index, logprob, dim, temperature, tail):
-        loss, aux = engine.distill_loss(student, index, logprob, dim, temperature, tail)
-        ctx.engine, ctx.args = engine, (dim, temperature, tail)
+        view = engine.logits_view(student, dim, "student")
+        loss, aux = engine.distill_loss(student, index, logprob, dim, temperature, tail, view)
+        ctx.call = engine, view, dim, temperature, tail
         ctx.save_for_backward(student, index, logprob, aux)
         return loss
 
@@ -182,7 +192,8 @@ class _DistillLoss(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_loss):
         student, index, logprob, aux = ctx.saved_tensors
-        return (ctx.engine.distill_backward(student, index, logprob, aux, g_loss, *ctx.args),) + (None,) * 6
+        engine, view, dim, temperature, tail = ctx.call
+        return (engine.distill_backward(student, index, logprob, aux, g_loss, dim, temperature, tail, view), None, None, None, None, None, None)
 
 
 def distill_loss(engine, student, teacher_index, teacher_logprob, dim: int = -1, temperature: float = 1.0, tail: bool = False) -> torch.Tensor:
