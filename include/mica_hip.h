@@ -241,7 +241,8 @@ int mica_neighbour_matrix_np(mica_ctx* ctx, const double* d_cands, int64_t n, co
 /* Rows of logits in any of three types, read where they are.  Row (o, i) begins at element o * stride_outer + i * stride_inner, its
  * class v lies stride_class * v further on.  class_last says how the results with a class or list axis are laid out: 1 = C-contiguous
  * [outer][inner][classes or K], 0 = [outer][classes or K][inner] (NCDHW logits of a head: outer = batch, inner = voxels).
- * More than 64 classes: class_last = 1 and stride_class = 1 only.  Limits: 1 <= classes <= 2^28, outer * inner < 2^31.          */
+ * More than 64 classes: class_last = 1 and stride_class = 1 only.  Limits: 1 <= classes <= 2^28, outer * inner < 2^31, and with more
+ * than 64 classes about 2^36 logits (what one launch covers).                                                                  */
 #define MICA_F32 0
 #define MICA_BF16 1
 #define MICA_F16 2

@@ -1433,7 +1433,9 @@ const char* logits_view(const mica_logits* z, LogitsView& v, int64_t& rows) {
     if (z->classes > SCORE_COL_MAX && (z->stride_class != 1 || !z->class_last)) return "more than 64 classes have to be contiguous and last";
     rows = z->outer * z->inner;
     if (rows > 0 && (!z->d_data || ((uintptr_t)z->d_data % (z->dtype == MICA_F32 ? 4 : 2)))) return "null or misaligned logits";
-    if (z->classes > SCORE_COL_MAX && rows * ((z->classes + SCORE_COL_MAX - 1) / 4096 + 1) > 0x7FFFFFFF) return "too many rows of this length";
+    // one launch has fewer than 2^32 threads: 256 for 1024 classes of four rows, or for 4096 of one
+    if (z->classes > SCORE_COL_MAX && (z->classes <= 4096 ? rows * ((z->classes + 1023) / 1024) / 4 : rows * ((z->classes + 4095) / 4096)) >= (1 << 24) - 1)
+        return "too many rows of this length for one call";
     v = LogitsView{z->d_data, z->dtype, z->class_last ? 1 : 0, z->outer, z->inner, z->classes, z->stride_outer, z->stride_inner, z->stride_class};
     return nullptr;
 }

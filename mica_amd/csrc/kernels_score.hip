@@ -710,11 +710,20 @@ struct RowGrad {
     float at_token;     // added at the token
     int64_t token;      // -1: none
     bool empty;
+    // |lse| > BIG (a row of the type's lowest values): lse is the maximum, float32 has lost the log of the sum; the classes that reach it
+    // share the row, one e^{-H} each, and every other one lies beyond any exponent
+    bool far;
+    float lse, inv_t, far_p, far_log2p;
 };
 __device__ __forceinline__ RowGrad row_grad(const ScoreGrad& o, int64_t classes, int64_t r) {
     RowGrad g;
     const float lse = o.lse[r];
     g.empty = lse == -INFINITY;
+    g.far = fabsf(lse) > BIG && !g.empty;
+    g.lse = lse;
+    g.inv_t = o.inv_t;
+    g.far_log2p = -o.entropy[r] * LOG2E;
+    g.far_p = exp2_hw(g.far_log2p);
     g.l2 = lse * LOG2E;
     float glp = 0.f;
     g.token = -1;
@@ -733,8 +742,12 @@ __device__ __forceinline__ RowGrad row_grad(const ScoreGrad& o, int64_t classes,
     return g;
 }
 __device__ __forceinline__ float grad_value(const RowGrad& g, float z, float c) {
-    const float x = fmaf(z, c, -g.l2);
-    const float p = exp2_hw(x);
+    float x = fmaf(z, c, -g.l2), p = exp2_hw(x);
+    if (g.far) {
+        const bool reaches = (float)((double)z * g.inv_t) == g.lse;
+        x = reaches ? g.far_log2p : NEG_BIG;
+        p = reaches ? g.far_p : 0.f;
+    }
     return g.empty ? 0.f : p * fmaf(g.b, fmaxf(x, NEG_BIG), g.a);
 }
 
@@ -789,12 +802,18 @@ struct DistillArgs {
     float c, inv_t, t;
     const float* weight;          // nullable: rows of weight 0 are skipped
     float* loss;
-    float* aux;                   // [4][rows], nullable: ref, factor, lse, mass (tail) or the teacher's log sum
+    float* aux;                   // [4][rows], nullable: RowGradient's m, f, M (tail) or norm, qs
     const float* g_loss;          // gradient kernels
 };
-// A row's gradient: factor * e^{y - ref} where a class is not listed, mass * e^{y - lse} - sum p at a listed one, times T and the
-// upstream gradient.  (tail: ref is the log sum of the classes that are not listed and factor = mass q_rest - r, so that nothing
-// overflows where q_rest is tiny; else ref = lse, factor = mass.)
+// A row's gradient, times T and the upstream gradient: (mass q_rest - r) times the share e^{y} / sum of e^{y} among the classes that are
+// not listed, for these (nothing overflows where q_rest is tiny), and mass q - sum p for the listed ones.  Both are kept relative to a
+// maximum, not to a log sum: a float32 log sum of a row of the type's lowest values would have lost the number of its classes.
+struct RowGradient {
+    float m, f;         // not listed: f 2^{z c - R(m)}, or f 2^{(z - m) c} beyond BIG
+    float M, qs;        // listed: qs 2^{(z - M) c} - sum p
+    float norm;         // log p = t - norm
+    __device__ __forceinline__ bool empty() const { return M == -INFINITY; }
+};
 // The row's list in LDS: index (unused entries -1, no class: INT_MAX), log probability, logit.  Loaded by one wave.
 struct ListLds { int* i; float* t; float* z; };
 constexpr unsigned LIST_BYTES = 12;                             // of LDS per entry
@@ -910,7 +929,7 @@ __device__ __forceinline__ ListStats list_stats(const DistillArgs& a, ListLds d,
 }
 // The row's scalars from its list and the sums over all classes, or over those that are not listed (tail); any thread.  What cancels is
 // combined in float64: 1 - sum p, log q_rest = -log(1 + listed sum / rest sum).
-struct RowScalars { double M, log_s, rest, log_q_rest, mass; float ref, factor, lse; };     // M, log_s: maximum and log sum of all classes
+struct RowScalars { double M, log_s, rest, log_q_rest, mass; RowGradient g; };     // M, log_s: maximum and log sum of all classes
 __device__ __forceinline__ RowScalars row_scalars(const DistillArgs& a, const ListStats& l, float m, float s) {
     RowScalars o;
     const double log_m = log_sum(m, s, a.c);                    // log of the streamed sum relative to m
@@ -919,11 +938,10 @@ __device__ __forceinline__ RowScalars row_scalars(const DistillArgs& a, const Li
     o.rest = o.log_q_rest = 0.0;
     o.mass = l.mass;
     const bool have_rest = !(s == 0.f);                         // NaN counts
-    double lse_rest = 0.0;
+    double factor = o.mass;
     if (a.tail) {
         o.rest = have_rest && l.mass < 1.0 ? 1.0 - l.mass : 0.0;
         o.mass += o.rest;
-        lse_rest = (double)m * a.inv_t + log_m;
         if (!have_rest) { o.M = l.zmax; o.log_s = l.log_sl; }
         else if (l.log_sl != -INFINITY) {
             o.M = fmaxf(m, l.zmax);
@@ -931,16 +949,15 @@ __device__ __forceinline__ RowScalars row_scalars(const DistillArgs& a, const Li
             o.log_q_rest = -(u > 700.0 ? u : log1p(exp(u)));
             o.log_s = ((double)m - o.M) * a.inv_t + log_m - o.log_q_rest;
         }
+        factor = o.mass * exp(o.log_q_rest) - o.rest;
     }
-    o.lse = s != s ? NAN : (o.M == -INFINITY ? -INFINITY : (float)(o.M * a.inv_t + o.log_s));
-    if (a.tail) {
-        o.ref = have_rest ? (float)lse_rest : 0.f;
-        o.factor = have_rest ? (float)(o.mass * exp(o.log_q_rest) - o.rest) : 0.f;
-    } else {
-        o.ref = o.lse;
-        o.factor = (float)o.mass;
-    }
-    if (l.bad || s != s) o.factor = NAN;                        // an invalid entry shows in the gradient too
+    const bool invalid = l.bad || s != s || o.log_s != o.log_s || o.mass != o.mass;      // shows in the gradient too
+    o.g.m = a.tail && !have_rest ? 0.f : m;                    // without a tail M itself
+    o.g.f = invalid ? NAN : (have_rest ? (float)(factor / s) : 0.f);
+    o.g.M = (float)o.M;
+    o.g.qs = invalid ? NAN : (o.M == -INFINITY ? 0.f : (float)(o.mass * exp(-o.log_s)));
+    o.g.norm = (float)l.norm;
+    if (invalid && o.M == -INFINITY) o.g.M = 0.f;               // a row of NaN is not an empty one
     return o;
 }
 // the loss; one wave, in every lane
@@ -957,21 +974,21 @@ __device__ __forceinline__ float row_loss(const DistillArgs& a, ListLds d, const
     if (o.rest > 0.0) sum += o.rest * (log(o.rest) - o.log_q_rest);
     return l.bad || s != s ? NAN : (float)(sum * a.t * a.t);
 }
-struct RowGradient { float ref, factor, lse, mass, norm; };
 // loss and aux of a row from its joined sums; one wave, the result in every lane
 __device__ __forceinline__ RowGradient finish_row(const DistillArgs& a, ListLds d, float m, float s, int64_t r, int64_t rows, int lane) {
     const ListStats l = list_stats(a, d, lane);
     const RowScalars o = row_scalars(a, l, m, s);
     const float loss = row_loss(a, d, l, o, s, lane);
-    const RowGradient q{o.ref, loss != loss ? NAN : o.factor, o.lse, (float)o.mass, (float)l.norm};
+    RowGradient q = o.g;
+    if (loss != loss) q.f = q.qs = NAN;
     if (lane == 0) {
         const float w = a.weight ? a.weight[r] : 1.f;
         a.loss[r] = w == 0.f ? 0.f : loss * w;
         if (a.aux) {
-            a.aux[r] = q.ref;
-            a.aux[rows + r] = q.factor;
-            a.aux[2 * rows + r] = q.lse;
-            a.aux[3 * rows + r] = a.tail ? q.mass : q.norm;
+            a.aux[r] = q.m;
+            a.aux[rows + r] = q.f;
+            a.aux[2 * rows + r] = a.tail ? q.M : q.norm;        // without a tail M = m
+            a.aux[3 * rows + r] = q.qs;
         }
     }
     return q;
@@ -1029,10 +1046,23 @@ __device__ __forceinline__ void listed_grad(const DistillArgs& a, T* __restrict_
             again |= j < k;
             p += a.tail ? expf(d.t[j]) : (q.norm == -INFINITY ? 0.f : expf(d.t[j] - q.norm));
         }
-        if (!again) out[i] = from_f32<T>(scale * (q.mass * exp2_hw(fmaf(d.z[k], a.c, -q.lse * LOG2E)) - p));
+        if (!again) out[i] = from_f32<T>(scale * (q.qs * exp2_hw((d.z[k] - q.M) * a.c) - p));
     }
 }
-__device__ __forceinline__ float unlisted_grad(float z, float ref2, float f, float c) { return f * exp2_hw(fmaf(z, c, -ref2)); }
+// the gradient of a class that is not listed
+struct Unlisted {
+    float sub, R, f, c;
+    bool none;
+    __device__ __forceinline__ Unlisted(const DistillArgs& a, const RowGradient& q, float scale) {
+        none = q.empty() || scale == 0.f;
+        const bool far = fabsf(q.m) > BIG;
+        sub = far ? q.m : 0.f;
+        R = far || none ? 0.f : reference(q.m, a.c);
+        f = none ? 0.f : scale * q.f;
+        c = a.c;
+    }
+    __device__ __forceinline__ float operator()(float z) const { return none ? 0.f : f * exp2_hw(fmaf(z - sub, c, -R)); }
+};
 
 template <typename T, int G, int ONCE>
 __global__ __launch_bounds__(256) void distill_grad_row_kernel(LogitsView v, int64_t rows, DistillArgs a, int chunks, T* __restrict__ grad) {
@@ -1050,13 +1080,12 @@ __global__ __launch_bounds__(256) void distill_grad_row_kernel(LogitsView v, int
     T* out = grad + r * v.classes;
     const float w = a.weight ? a.weight[r] : 1.f;
     const float scale = (a.g_loss ? a.g_loss[r] : 1.f) * w * a.t;
-    const float x = a.aux[3 * rows + r];
-    const RowGradient o{a.aux[r], a.aux[rows + r], a.aux[2 * rows + r], a.tail ? x : (x == -INFINITY ? 0.f : 1.f), a.tail ? 0.f : x};
-    const bool none = o.lse == -INFINITY || w == 0.f;
-    const float ref2 = none ? 0.f : o.ref * LOG2E, f = none ? 0.f : scale * o.factor;
-    map_chunk<T, G, ONCE>(z, out, first, v.classes, tid, [&](float y, int64_t) { return none ? 0.f : unlisted_grad(y, ref2, f, a.c); });
+    const float x = a.aux[2 * rows + r], m = a.aux[r];
+    const RowGradient o{m, a.aux[rows + r], a.tail ? x : m, a.aux[3 * rows + r], a.tail ? 0.f : x};
+    const Unlisted unlisted(a, o, scale);
+    map_chunk<T, G, ONCE>(z, out, first, v.classes, tid, [&](float y, int64_t) { return unlisted(y); });
     group_sync<G>();
-    if (!none) listed_grad<T, G>(a, out, list, first, CHUNK, o, scale, tid);
+    if (!unlisted.none) listed_grad<T, G>(a, out, list, first, CHUNK, o, scale, tid);
 }
 
 // Loss and gradient in one kernel: the row is read twice, the second time from cache, and its gradient written.  So that the second
@@ -1092,12 +1121,11 @@ __global__ __launch_bounds__(G < 256 ? 256 : G, 8) void distill_step_kernel(Logi
         o = shared_row[g];
     }
     const float scale = a.t * (a.weight ? a.weight[r] : 1.f);
-    const bool none = o.lse == -INFINITY || scale == 0.f;
-    const float ref2 = none ? 0.f : o.ref * LOG2E, f = none ? 0.f : scale * o.factor;
+    const Unlisted unlisted(a, o, scale);
     const auto put = [&](const float(&y)[N], int vec) {
         float d[N];
 #pragma unroll
-        for (int j = 0; j < N; ++j) d[j] = none ? 0.f : unlisted_grad(y[j], ref2, f, a.c);
+        for (int j = 0; j < N; ++j) d[j] = unlisted(y[j]);
         if (vec < n / N) store_vec<ONCE != ONCE_NONE>(out + (int64_t)vec * N, d);
         else if (vec * N < n) {
             const int shift = edge_shift<T>(n, vec);
@@ -1118,7 +1146,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G, 8) void distill_step_kernel(Logi
         },
         put);
     group_sync<G>();
-    if (!none) listed_grad<T, G>(a, out, list, 0, n, o, scale, tid);
+    if (!unlisted.none) listed_grad<T, G>(a, out, list, 0, n, o, scale, tid);
 }
 
 // ========================================================================================================================================

@@ -562,3 +562,67 @@ def test_candidates_residues_and_a_student_of_the_network(weights):
     wl, wg, _ = so.distill(student.detach().cpu().movedim(1, -1), s.top_index.cpu().movedim(1, -1), s.top_logprob.cpu().movedim(1, -1), 1.0, True)
     assert abs(float(loss.detach()) - float(wl.mean())) < 1e-5
     assert float((student.grad.cpu().double() - wg.movedim(-1, 1) / 4096).abs().max()) < 1e-5 / 4096
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("classes", [7, 64, 300, 5000, 70001])
+def test_rows_of_the_lowest_value_are_uniform_in_the_gradients_too(eng, dtype, classes):
+    """a row masked with finfo.min throughout, or but for two classes: float32 log sums of it are the lowest value itself"""
+    low = torch.finfo(DT[dtype]).min
+    z = torch.full((3, classes), low).to(DT[dtype])
+    z[1, ::2] = NEG
+    z[2] = NEG
+    z[2, [1, classes - 1]] = low
+    tok = torch.tensor([1, 2, classes - 1])
+    g = torch.tensor([1.0, -2.0, 0.5])
+    for temperature in (1.0, 0.9 if dtype == "f16" else 1.25):
+        d = z.cuda()
+        r = eng.token_logprobs(d, tok.cuda(), temperature=temperature)
+        got = eng.token_logprobs_backward(d, tok.cuda(), r.lse, r.entropy, g.cuda(), g.cuda(), temperature=temperature)
+        want = so.score_grad(z, tok, g, g, None, temperature)
+        # f16: lse = -65504 + log C is rounded to a float32 of step 2^-8 (relative 2^-24), which the exponentials see in full
+        rel = U * (64 + classes / 64) + (2.0 ** -8 if dtype == "f16" else 0.0)
+        _near(got, want, rel * (want.abs() + 4.0 * g.abs()[:, None] / classes) * 4 + _half_step(dtype, want) + 1e-37)
+        k = min(4, classes)
+        idx = torch.arange(k).repeat(3, 1).int()
+        val = torch.log(torch.tensor([0.4, 0.3, 0.1, 0.05])[:k]).repeat(3, 1)
+        for tail in (False, True):
+            if not tail:                                     # the list names classes the last two rows forbid: +inf there
+                wl, wg, _ = so.distill(z[:1], idx[:1], val[:1], temperature, tail)
+                zz, ii, vv, gg = d[:1], idx[:1].cuda(), val[:1].cuda(), g[:1]
+            else:
+                ii = torch.full_like(idx, -1)
+                ii[0] = idx[0]
+                ii[1, 0], ii[2, 0] = 1, classes - 1
+                wl, wg, _ = so.distill(z, ii, val, temperature, tail)
+                zz, ii, vv, gg = d, ii.cuda(), val.cuda(), g
+            loss, aux = eng.distill_loss(zz, ii, vv, temperature=temperature, tail=tail)
+            got = eng.distill_backward(zz, ii, vv, aux, gg.cuda(), temperature=temperature, tail=tail)
+            want = wg * gg.double()[:, None]
+            tol = U * (64 + classes / 64 + 8 * _log2c(classes)) * 4
+            _near(loss, wl, tol * (1 + wl.abs()) * temperature ** 2)
+            _near(got, want, tol * (want.abs() + 2.0 / classes) * temperature + _half_step(dtype, want) + 1e-37)
+            sl, sg = eng.distill_step(zz, ii, vv, temperature=temperature, tail=tail, weight=gg.cuda())
+            _near(sg, want, tol * (want.abs() + 2.0 / classes) * temperature + _half_step(dtype, want) + 1e-37)
+
+
+def test_autograd_rules(eng):
+    """written-to inputs and second derivatives are refused, not answered wrongly"""
+    from mica_amd import scoring
+    z = _logits((4, 300), 1, "f32").cuda()
+    tok = torch.zeros(4, dtype=torch.int64, device="cuda")
+    idx, val = _teacher(z.cpu(), 3, 2)
+    for make in (lambda x: scoring.token_logprobs(eng, x, tok).logprob, lambda x: scoring.distill_loss(eng, x, idx.cuda(), val.cuda())):
+        x = z.clone().requires_grad_()
+        y = x * 1.0
+        out = make(y).sum()
+        with torch.no_grad():
+            y.mul_(2.0)
+        with pytest.raises(RuntimeError):
+            out.backward()
+        x = z.clone().requires_grad_()
+        g, = torch.autograd.grad(make(x).sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError):
+            g.sum().backward()
+    r = scoring.token_logprobs(eng, z.clone().requires_grad_(), tok, top=2)
+    assert not r.top_logprob.requires_grad and not r.top_index.requires_grad and r.lse.requires_grad
