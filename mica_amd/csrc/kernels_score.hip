@@ -372,9 +372,10 @@ template <typename T, int G, int U, int ONCE, typename F, typename H> __device__
 // The K <= 64 largest of a group's row.  While streaming, every thread notes its largest value and the vector that held it first.  Of
 // these (value, position) pairs each wave takes its ceil(K / waves)-th largest; the smallest of those bounds the K-th largest element
 // from below, so only threads at or above the bound can own one of the K.  A long row is noted in PARTS stretches, and only the stretches
-// at or above the bound are read once more (about K / (PARTS G) of the row) and what passes the bound is sorted, one key per lane.  More than 64 pass only in unusual data (many equal values, everything
-// large in one place); then every wave merges its share, 64 keys at a time, into a sorted list.  Exact for any data; ties and -inf order
-// by index.
+// at or above the bound are read once more (about K / (PARTS G) of the row; 4096 x 128000 bf16, K = 20: 272 us with one stretch, 227 with
+// four) and what passes the bound is sorted, one key per lane.  More than 64 pass only for K near 64 or in unusual data (many equal
+// values, everything large in one place); then every wave merges its share, 64 keys at a time, into a sorted list.  Exact for any data;
+// ties and -inf order by index.
 struct TopScratch {             // LDS of one wave
     u64 list[64];
     u64 buf[128];
@@ -586,6 +587,9 @@ __device__ __forceinline__ void write_top(const ScoreOut& o, const LogitsView& v
     }
 }
 
+// One read of the logits.  HBM-bound without alternatives: 4096 x 128000 bf16 175 us = 6.0 TB/s (a bare read of it 152-175 us), 7.6
+// instructions and one exponential per logit, half of the issue slots.  With alternatives the selection behind the stream is not hidden
+// by the other blocks of the CU: 227 us for K = 20.  Two vectors at a time then, which leaves registers for six blocks.
 template <typename T, int G, bool TOP, int ONCE>
 __global__ __launch_bounds__(256) void score_row_kernel(LogitsView v, int64_t rows, ScoreOut o, int segments, int seg_len, Partial* __restrict__ part,
                                                         u64* __restrict__ part_top) {
@@ -691,7 +695,8 @@ __global__ __launch_bounds__(TOP ? JOIN : 64) void score_join_kernel(LogitsView 
 }
 
 // ---- gradient of the scores ------------------------------------------------------------------------------------------------------------
-// dz_v = (1/T) [ g_lp ([v = t] - p_v) + g_lse p_v - g_H p_v (log p_v + H) ]: one read, one write, no state but lse and H
+// dz_v = (1/T) [ g_lp ([v = t] - p_v) + g_lse p_v - g_H p_v (log p_v + H) ]: one read, one write, no state but lse and H.  HBM-bound:
+// 4096 x 32000 bf16 89 us = 5.9 TB/s, above the rate of a copy because the forward pass left part of the logits in the Infinity Cache.
 struct ScoreGrad {
     const void* tokens;
     int token_bytes;
@@ -741,12 +746,15 @@ __device__ __forceinline__ RowGrad row_grad(const ScoreGrad& o, int64_t classes,
     g.at_token = g.empty ? 0.f : glp * o.inv_t;
     return g;
 }
-__device__ __forceinline__ float grad_value(const RowGrad& g, float z, float c) {
-    float x = fmaf(z, c, -g.l2), p = exp2_hw(x);
-    if (g.far) {
+template <bool FAR> __device__ __forceinline__ float grad_value(const RowGrad& g, float z, float c) {
+    float x, p;
+    if (FAR) {
         const bool reaches = (float)((double)z * g.inv_t) == g.lse;
         x = reaches ? g.far_log2p : NEG_BIG;
         p = reaches ? g.far_p : 0.f;
+    } else {
+        x = fmaf(z, c, -g.l2);
+        p = exp2_hw(x);
     }
     return g.empty ? 0.f : p * fmaf(g.b, fmaxf(x, NEG_BIG), g.a);
 }
@@ -787,8 +795,13 @@ __global__ __launch_bounds__(256) void score_grad_row_kernel(LogitsView v, int64
     const int first = chunks == 1 ? 0 : (int)(item % chunks) * CHUNK;
     const RowGrad g = row_grad(o, v.classes, r);
     const T* z = static_cast<const T*>(v.p) + row_start(v, row_pos(v, r));
-    map_chunk<T, G, ONCE>(z, grad + r * v.classes, first, v.classes, tid,
-                    [&](float x, int64_t at) { return grad_value(g, x, o.c) + (at == g.token ? g.at_token : 0.f); });
+    const auto chunk = [&](auto far) {
+        map_chunk<T, G, ONCE>(z, grad + r * v.classes, first, v.classes, tid, [&](float x, int64_t at) {
+            return grad_value<decltype(far)::value>(g, x, o.c) + (at == g.token ? g.at_token : 0.f);
+        });
+    };
+    if (__builtin_expect(g.far, 0)) chunk(std::true_type());
+    else chunk(std::false_type());
 }
 
 // ---- distillation ------------------------------------------------------------------------------------------------------------------------
@@ -799,7 +812,8 @@ struct DistillArgs {
     int teacher_dtype;
     int k;
     int tail;
-    float c, inv_t, t;
+    float c, t;
+    double inv_t;                 // of the few terms that are combined in float64
     const float* weight;          // nullable: rows of weight 0 are skipped
     float* loss;
     float* aux;                   // [4][rows], nullable: RowGradient's m, f, M (tail) or norm, qs
@@ -994,6 +1008,8 @@ __device__ __forceinline__ RowGradient finish_row(const DistillArgs& a, ListLds 
     return q;
 }
 
+// One read of the logits, a bit of LDS per class to leave out the listed ones (tail; subtracting them afterwards would cancel for every
+// good student).  HBM-bound: 4096 x 128000 bf16 174 us = 6.0 TB/s, 180 with the tail; 513 x 32003 15 us, the latency of its steps.
 template <typename T, int G, bool TAIL, int ONCE>
 __global__ __launch_bounds__(256) void distill_row_kernel(LogitsView v, int64_t rows, DistillArgs a, int segments, int seg_len, Partial* __restrict__ part) {
     constexpr int GROUPS = 256 / G;
@@ -1064,6 +1080,7 @@ struct Unlisted {
     __device__ __forceinline__ float operator()(float z) const { return none ? 0.f : f * exp2_hw(fmaf(z - sub, c, -R)); }
 };
 
+// One read, one write: 1999 x 65537 f16 92 us = 5.7 TB/s.
 template <typename T, int G, int ONCE>
 __global__ __launch_bounds__(256) void distill_grad_row_kernel(LogitsView v, int64_t rows, DistillArgs a, int chunks, T* __restrict__ grad) {
     constexpr int GROUPS = 256 / G, CHUNK = G * UNROLL * Vec<T>::N;
@@ -1089,7 +1106,9 @@ __global__ __launch_bounds__(256) void distill_grad_row_kernel(LogitsView v, int
 }
 
 // Loss and gradient in one kernel: the row is read twice, the second time from cache, and its gradient written.  So that the second
-// read finds it there, G is chosen to leave few rows in flight: 2048 / G blocks on a CU.
+// read finds it there, G is chosen to leave few rows in flight: 2048 / G blocks on a CU (step_group).  4096 x 128000 bf16 489 us = 4.3 TB/s
+// of one read and one write; the two-kernel form takes 174 + 400, 256 threads per row 662 (the second read from HBM).  Holding the row in
+// the registers of 1024 threads took 562: one block on a CU, nothing to do while it sums.
 constexpr int STEP_U = 2;                                       // 64 registers: two blocks of 1024 threads on a CU
 template <typename T, int G, bool TAIL, int ONCE>
 __global__ __launch_bounds__(G < 256 ? 256 : G, 8) void distill_step_kernel(LogitsView v, int64_t rows, DistillArgs a, T* __restrict__ grad) {
@@ -1150,7 +1169,9 @@ __global__ __launch_bounds__(G < 256 ? 256 : G, 8) void distill_step_kernel(Logi
 }
 
 // ========================================================================================================================================
-// rows of few classes, at any stride: a thread per row, the classes in registers
+// rows of few classes, at any stride: a thread per row, the classes in registers.  8 x 20 x 64^3 f32 scores with three alternatives 54 us
+// = 4.8 TB/s, the gradient of 4 x 21 x 64^3 32 us = 5.5 TB/s; the distillation, whose list costs every class a comparison, is bound by its
+// instructions: loss 43 us, gradient 55 us for 4 x 21 x 64^3 with four entries.
 // ========================================================================================================================================
 template <int CM, typename T> __device__ __forceinline__ void load_classes(float (&z)[CM], const T* p, int64_t sc, int classes) {
 #pragma unroll
@@ -1212,11 +1233,11 @@ __global__ __launch_bounds__(256) void score_grad_col_kernel(LogitsView v, int64
     const int64_t step = v.class_last ? 1 : v.inner;
 #pragma unroll
     for (int c = 0; c < CM; ++c)
-        if (c < classes) out[c * step] = from_f32<T>(grad_value(g, z[c], o.c) + (c == g.token ? g.at_token : 0.f));
+        if (c < classes) out[c * step] = from_f32<T>((g.far ? grad_value<true>(g, z[c], o.c) : grad_value<false>(g, z[c], o.c)) + (c == g.token ? g.at_token : 0.f));
 }
 
-// Loss (a.loss) and / or gradient (grad) of a row; the gradient's scale: weight or the upstream gradient.  In float32 but for 1 - sum p,
-// which cancels: a few classes leave sums of a few roundings.  The exponentials relative to the row's maximum are kept for the gradient
+// Loss (a.loss) and / or gradient (grad) of a row; the gradient's scale: weight or the upstream gradient.  In float32, as a few classes
+// leave sums of a few roundings, but for what cancels: 1 - sum p, and the loss of a good student.  The exponentials relative to the row's maximum are kept for the gradient
 // (recomputed relative to the rest's maximum where the rest would underflow).
 template <typename T, int CM, bool LOSS, bool GRAD>
 __global__ __launch_bounds__(256) void distill_col_kernel(LogitsView v, int64_t rows, DistillArgs a, T* __restrict__ grad) {
@@ -1255,10 +1276,10 @@ __global__ __launch_bounds__(256) void distill_col_kernel(LogitsView v, int64_t 
         target[c] = 0.f;
     }
     const bool empty = m == -INFINITY;
-    const float log_s = logf(s);
+    const double log_s = LOSS ? log((double)s) : (double)logf(s);
     u64 listed = 0;
     bool bad = false;
-    float sum = 0.f;
+    double sum = 0.0;
     for (int k = 0; k < a.k; ++k) {
         const int64_t i = load_int(a.index, l.base + k * l.stride, a.index_bytes);
         if (i < 0) continue;
@@ -1272,9 +1293,10 @@ __global__ __launch_bounds__(256) void distill_col_kernel(LogitsView v, int64_t 
             zk = c == (int)i ? z[c] : zk;
             target[c] += c == (int)i ? pk : 0.f;
         }
-        if (LOSS && !(pk == 0.f)) sum += pk * (lp - (empty ? -INFINITY : fmaf(zk - m, a.inv_t, -log_s)));
+        if (LOSS && !(pk == 0.f)) sum += pk * (lp - (empty ? -INFINITY : (double)(zk - m) * a.inv_t - log_s));
     }
-    float mass = nobody ? 0.f : 1.f, rest = 0.f, log_q_rest = 0.f, s_rest = 0.f;
+    float mass = nobody ? 0.f : 1.f, rest = 0.f, s_rest = 0.f;
+    double log_q_rest = 0.0;
     if (a.tail) {
         float m_rest = -INFINITY;
 #pragma unroll
@@ -1283,9 +1305,9 @@ __global__ __launch_bounds__(256) void distill_col_kernel(LogitsView v, int64_t 
             m_rest = fmaxf(m_rest, in ? -INFINITY : z[c]);
             s_rest += in ? 0.f : e[c];
         }
-        float shift = 0.f;
+        double shift = 0.0;
         if (m_rest > -INFINITY && (m_rest - m) * a.c < -60.f) {             // far below the listed ones: relative to its own maximum
-            shift = (m_rest - m) * a.inv_t;
+            shift = ((double)m_rest - m) * a.inv_t;
             s_rest = 0.f;
 #pragma unroll
             for (int c = 0; c < CM; ++c) {
@@ -1297,15 +1319,15 @@ __global__ __launch_bounds__(256) void distill_col_kernel(LogitsView v, int64_t 
         }
         rest = s_rest > 0.f && total < 1.0 ? (float)(1.0 - total) : 0.f;
         if (!(rest > 0.f)) mass = (float)total;
-        log_q_rest = shift + logf(s_rest) - log_s;
-        if (LOSS && rest > 0.f) sum += rest * (logf(rest) - log_q_rest);
+        log_q_rest = shift + (LOSS ? log((double)s_rest) : (double)logf(s_rest)) - log_s;
+        if (LOSS && rest > 0.f) sum += rest * (log((double)rest) - log_q_rest);
     }
     const bool nan = bad || s != s || sum != sum;
-    if (LOSS) a.loss[r] = w == 0.f ? 0.f : (nan ? NAN : sum * a.t * a.t) * w;
+    if (LOSS) a.loss[r] = w == 0.f ? 0.f : (nan ? NAN : (float)(sum * a.t * a.t)) * w;
     if (GRAD) {
         const float scale = (a.g_loss ? a.g_loss[r] : 1.f) * w * a.t;
         const bool none = empty || w == 0.f;
-        const float in_f = scale * mass / s, out_f = a.tail ? (s_rest > 0.f ? scale * (mass * expf(log_q_rest) - rest) / s_rest : 0.f) : in_f;
+        const float in_f = scale * mass / s, out_f = a.tail ? (s_rest > 0.f ? scale * (mass * expf((float)log_q_rest) - rest) / s_rest : 0.f) : in_f;
         T* out = grad + grad_start(v, p, r);
         const int64_t step = v.class_last ? 1 : v.inner;
 #pragma unroll
@@ -1499,7 +1521,7 @@ static DistillArgs distill_args(const DistillList& d, float temperature) {
     a.k = d.k;
     a.tail = d.tail;
     a.c = LOG2E / temperature;
-    a.inv_t = 1.0f / temperature;
+    a.inv_t = 1.0 / temperature;
     a.t = temperature;
     return a;
 }
