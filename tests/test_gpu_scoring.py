@@ -626,3 +626,14 @@ def test_autograd_rules(eng):
             g.sum().backward()
     r = scoring.token_logprobs(eng, z.clone().requires_grad_(), tok, top=2)
     assert not r.top_logprob.requires_grad and not r.top_index.requires_grad and r.lse.requires_grad
+
+
+@pytest.mark.parametrize("rows,classes,dtype", [(260, 66003, "f32"), (257, 131080, "bf16")])
+def test_many_rows_longer_than_one_block_takes(eng, rows, classes, dtype):
+    """rows enough for a block each, but longer than its bits cover: still cut, and distill_step in two kernels"""
+    z = _logits((rows, classes), 3, dtype)
+    tok = torch.randint(0, classes, (rows,), generator=_rng(5))
+    _check_score(eng, z, tok, 9)
+    idx, val = _teacher(z, 12, 6)
+    for tail in (False, True):
+        _check_distill(eng, z, idx, val, dtype, 1.0, tail)
