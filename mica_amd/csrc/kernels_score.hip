@@ -544,6 +544,8 @@ __device__ __forceinline__ u64 group_top(const T* __restrict__ z, int n, unsigne
     return list == 0 ? 0 : ((list & 0xFFFFFFFF00000000ull) | (0xFFFFFFFFu - (key_index(list) + index0)));
 }
 
+// -inf is kept for rows without a class: a log sum of -3.4e38 / T, T < 1, is the lowest value
+__device__ __forceinline__ float finite(float x) { return fminf(fmaxf(x, -3.402823466e38f), 3.402823466e38f); }
 // a row's results from its joined sums; one thread
 struct ScoreOut {
     const void* tokens;
@@ -565,7 +567,7 @@ template <typename L> __device__ __forceinline__ float class_logprob(float z, fl
 template <typename T, typename L>
 __device__ __forceinline__ void write_row(const ScoreOut& o, const T* __restrict__ z, int64_t sc, int64_t classes, int64_t r, float m, float s, float w,
                                           L log_s) {
-    o.lse[r] = s != s ? s : (m == -INFINITY ? -INFINITY : (float)((L)m * o.inv_t + log_s));
+    o.lse[r] = s != s ? s : (m == -INFINITY ? -INFINITY : finite((float)((L)m * o.inv_t + log_s)));
     // log2 s - w / s in the units of R cancels nothing: both parts of the entropy are >= 0 up to rounding
     const L log2_s = sizeof(L) == 8 ? (L)log2((double)s) : (L)log2f(s);
     const float h = s == 0.f ? 0.f : (float)((L)LN2 * (log2_s - (L)w / (L)s));
@@ -749,7 +751,7 @@ __device__ __forceinline__ RowGrad row_grad(const ScoreGrad& o, int64_t classes,
 template <bool FAR> __device__ __forceinline__ float grad_value(const RowGrad& g, float z, float c) {
     float x, p;
     if (FAR) {
-        const bool reaches = (float)((double)z * g.inv_t) == g.lse;
+        const bool reaches = z != -INFINITY && finite((float)((double)z * g.inv_t)) == g.lse;
         x = reaches ? g.far_log2p : NEG_BIG;
         p = reaches ? g.far_p : 0.f;
     } else {

@@ -575,7 +575,7 @@ def test_rows_of_the_lowest_value_are_uniform_in_the_gradients_too(eng, dtype, c
     z[2, [1, classes - 1]] = low
     tok = torch.tensor([1, 2, classes - 1])
     g = torch.tensor([1.0, -2.0, 0.5])
-    for temperature in (1.0, 0.9 if dtype == "f16" else 1.25):
+    for temperature in (1.0, 0.7, 0.9 if dtype == "f16" else 1.25):
         d = z.cuda()
         r = eng.token_logprobs(d, tok.cuda(), temperature=temperature)
         got = eng.token_logprobs_backward(d, tok.cuda(), r.lse, r.entropy, g.cuda(), g.cuda(), temperature=temperature)
@@ -637,3 +637,69 @@ def test_many_rows_longer_than_one_block_takes(eng, rows, classes, dtype):
     idx, val = _teacher(z, 12, 6)
     for tail in (False, True):
         _check_distill(eng, z, idx, val, dtype, 1.0, tail)
+
+
+def test_c_entry_points_refuse_on_the_host(eng):
+    """through the C ABI with a real context: refused with a message, nothing launched, the next call unharmed"""
+    import ctypes as C
+    from mica_amd import _cabi, scoring
+    z = torch.randn((3, 40000), generator=_rng(1)).cuda()
+    v = scoring.LogitsLayout(z, 1)
+    f = torch.empty(3, device="cuda")
+    tok = torch.zeros(3, dtype=torch.int64, device="cuda")
+    need = eng.lib.mica_token_logprobs_ws(C.byref(v.desc), 0)
+    ws = torch.empty(max(need, 16) + 16, dtype=torch.uint8, device="cuda")
+    p = lambda t: t.data_ptr()
+    assert need > 0
+    ok = (eng._h, C.byref(v.desc), p(tok), 8, -100, 1.0, 0, p(f), p(f), p(f), None, None, p(ws), need, eng._raw_stream())
+    bad = {1: None, 2: None, 3: 3, 5: 0.0, 6: 65, 7: None, 8: None, 9: None, 12: None, 13: need - 1}
+    for at, value in bad.items():
+        args = list(ok)
+        args[at] = value
+        assert eng.lib.mica_token_logprobs(*args) == _cabi.MICA_ERR_ARG, at
+        assert b"mica_token_logprobs" in eng.lib.mica_last_error(eng._h)
+    args = list(ok)
+    args[12] += 8                                            # misaligned
+    assert eng.lib.mica_token_logprobs(*args) == _cabi.MICA_ERR_ARG
+    args = list(ok)
+    args[6] = 3                                              # alternatives without a place to write them
+    assert eng.lib.mica_token_logprobs(*args) == _cabi.MICA_ERR_ARG
+    idx = torch.zeros((3, 2), dtype=torch.int32, device="cuda")
+    val = torch.zeros((3, 2), device="cuda")
+    for kw in (dict(k=0), dict(k=257), dict(index_bytes=2), dict(value_dtype=7), dict(d_index=None), dict(d_value=None)):
+        d = dict(d_index=p(idx), d_value=p(val), index_bytes=4, value_dtype=0, k=2, tail=0)
+        d.update(kw)
+        lst = _cabi.MicaTopList(*[d[n] for n, _ in _cabi.MicaTopList._fields_])
+        assert eng.lib.mica_distill_loss(eng._h, C.byref(v.desc), C.byref(lst), 1.0, p(f), None, p(ws), need, eng._raw_stream()) == _cabi.MICA_ERR_ARG
+        assert b"mica_distill_loss" in eng.lib.mica_last_error(eng._h)
+    lst = _cabi.MicaTopList(p(idx), p(val), 4, 0, 2, 0)
+    assert eng.lib.mica_distill_backward(eng._h, C.byref(v.desc), C.byref(lst), 1.0, None, p(f), p(z), eng._raw_stream()) == _cabi.MICA_ERR_ARG
+    assert eng.lib.mica_distill_step(eng._h, C.byref(v.desc), C.byref(lst), 1.0, None, p(f), None, p(ws), need, eng._raw_stream()) == _cabi.MICA_ERR_ARG
+    assert eng.lib.mica_token_logprobs(*ok) == 0
+    torch.cuda.synchronize()
+
+
+def test_two_threads_share_an_engine(eng):
+    """each on a stream of its own; the workspaces of their calls are their own as well"""
+    import threading
+    sets = []
+    for seed in (1, 2):
+        z = _logits((2, 60000), seed, "bf16")
+        idx, val = _teacher(z, 5, seed)
+        sets.append([t.cuda() for t in (z, torch.randint(0, 60000, (2,), generator=_rng(seed)), idx, val, torch.rand((2,), generator=_rng(2)))])
+    want = [_all_outputs(eng, *s) for s in sets]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = _all_outputs(eng, *sets[i])
+            torch.cuda.current_stream().synchronize()
+            wrong.extend(not torch.equal(a, b) for a, b in zip(got, want[i]))
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(wrong) == 2 * len(want[0]) and not any(wrong)
