@@ -401,7 +401,8 @@ class Engine:
         logprob (of `tokens`, integers of the logits' shape without `dim`; ignore_index: 0, any other value outside [0, classes): NaN),
         entropy and lse (log sum exp), all float32; top_logprob float32 / top_index int32, the `top` (<= 64) most probable classes in
         order, ties to the lowest class.  Logits float32, bfloat16 or float16 of any strides.  A row whose classes are all -inf: log
-        probabilities and lse -inf, entropy 0 (any other row's lse is kept within float32).  Asynchronous; the results have no autograd history (scoring.token_logprobs has)."""
+        probabilities and lse -inf, entropy 0 (any other row's lse is kept within float32).  Asynchronous; the results have no autograd
+        history (scoring.token_logprobs has)."""
         v = self.logits_view(logits, dim) if view is None else view
         temperature = scoring.check_temperature(temperature)
         top = int(top)
