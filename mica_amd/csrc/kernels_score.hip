@@ -183,25 +183,31 @@ __device__ __forceinline__ u64 lane_key(u64 v, int l) {             // of a lane
 }
 
 // ---- online softmax of one thread -----------------------------------------------------------------------------------------------------
-// m: running maximum;  s = sum 2^{z c - R}, w = sum 2^{z c - R} (z c - R) with the reference R = m c rounded to float32.  One fma per
-// logit, and R being off by a rounding cancels: whoever reads s uses the same R (reference(), log_sum()).  Beyond |m| = BIG, where m c
-// may overflow (a row of the type's lowest values), the sums are relative to m c itself and the exponents (z - m) c.
-constexpr float BIG = 1.0e30f;
+// m: running maximum;  s = sum 2^{z c - R}, w = sum 2^{z c - R} (z c - R) with the reference R = m c rounded to float32: one fma per logit.
+// R's rounding, up to half a step of R, is part of every exponent; it cancels, because whoever reads s uses the same R (ref_step(),
+// log_sum()), as long as it is small itself.  So beyond |R| = REF_MAX (rounding 1/16; rows masked throughout with -1e9, say) the sums are
+// relative to m c itself and the exponents (z - m) c: two instructions.  That is asked of the thread's maximum, at every one that it passes.
+constexpr float REF_MAX = 1048576.0f;
+constexpr float REF_STEP = 256.0f;                           // 2^-REF_STEP is 0
 __device__ __forceinline__ float reference(float m, float c) {
 #pragma clang fp contract(off)
     return m * c;
 }
+__device__ __forceinline__ bool ref_near(float R) { return fabsf(R) <= REF_MAX; }      // not for an infinite maximum
+// exponent of the maximum itself
+__device__ __forceinline__ float ref_residue(float m, float c) {
+    const float R = reference(m, c);
+    return ref_near(R) ? fmaf(m, c, -R) : 0.f;
+}
 // exponent between the references of two maxima, old <= now; -inf - -inf and the like end at NEG_BIG (with empty sums)
 __device__ __forceinline__ float ref_step(float old, float now, float c) {
 #pragma clang fp contract(off)
-    const float d = !(fabsf(old) <= BIG) || !(fabsf(now) <= BIG) ? (old - now) * c : reference(old, c) - reference(now, c);
+    const float a = reference(old, c), b = reference(now, c);
+    const float d = ref_near(a) && ref_near(b) ? a - b : (old - now) * c + (ref_residue(now, c) - ref_residue(old, c));
     return fmaxf(d, NEG_BIG);
 }
 // log of sum_v e^{(z_v - m) / T}; -inf for an empty row
-__device__ __forceinline__ double log_sum(float m, double s, float c) {
-    const double l = log(s);
-    return fabsf(m) <= BIG ? l + ((double)reference(m, c) - (double)m * c) * LN2 : l;
-}
+__device__ __forceinline__ double log_sum(float m, double s, float c) { return log(s) - (double)ref_residue(m, c) * LN2; }
 struct Online {
     float m = -INFINITY, s = 0.f, w = 0.f;
     // to a maximum >= m
@@ -224,22 +230,22 @@ struct Online {
     }
     // N logits, vmax their maximum (never NaN).  All lanes of a wave call it together.
     template <int N, bool ENT> __device__ __forceinline__ void add(const float (&f)[N], float vmax, float c) {
-        const float mn = fmaxf(m, vmax);
-        if (__builtin_expect(__any(!(fabsf(mn) <= BIG)), 0)) {       // some lane's maximum is -inf, or beyond BIG
+        const float mn = fmaxf(m, vmax), R = reference(mn, c), old = reference(m, c);
+        // some lane's maximum is -inf or of large magnitude, or was so and its sums still count
+        if (__builtin_expect(__any(!ref_near(R) || !ref_near(fmaxf(old, R - REF_STEP))), 0)) {
             rescale(mn, c);
-            const bool far = !(fabsf(mn) <= BIG) && mn != -INFINITY;
-            const float R = far || mn == -INFINITY ? 0.f : reference(mn, c), sub = far ? mn : 0.f;
+            const bool none = mn == -INFINITY, far = !ref_near(R) && !none;
+            const float ref = far || none ? 0.f : R, sub = far ? mn : 0.f;
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                const float x = far ? (f[j] - sub) * c : fmaf(f[j], c, -R);
+                const float x = far ? (f[j] - sub) * c : fmaf(f[j], c, -ref);
                 const float e = exp2_hw(x);
                 s += e;
                 if (ENT) w = fmaf(e, fmaxf(x, NEG_BIG), w);
             }
             return;
         }
-        const float R = reference(mn, c);
-        const float d = fmaxf(reference(m, c) - R, NEG_BIG);
+        const float d = fmaxf(old - R, NEG_BIG);
         const float a = exp2_hw(d);
         if (ENT) w = a * fmaf(s, d, w);
         s *= a;
@@ -710,6 +716,7 @@ struct ScoreGrad {
     const float* g_lse;
     float c, inv_t;
 };
+constexpr float BIG = 1.0e30f;
 struct RowGrad {
     float l2;           // lse in units of log 2
     float a;            // coefficient of p
@@ -825,7 +832,7 @@ struct DistillArgs {
 // not listed, for these (nothing overflows where q_rest is tiny), and mass q - sum p for the listed ones.  Both are kept relative to a
 // maximum, not to a log sum: a float32 log sum of a row of the type's lowest values would have lost the number of its classes.
 struct RowGradient {
-    float m, f;         // not listed: f 2^{z c - R(m)}, or f 2^{(z - m) c} beyond BIG
+    float m, f;         // not listed: f 2^{z c - R(m)}, or f 2^{(z - m) c} beyond REF_MAX
     float M, qs;        // listed: qs 2^{(z - M) c} - sum p
     float norm;         // log p = t - norm
     __device__ __forceinline__ bool empty() const { return M == -INFINITY; }
@@ -1073,7 +1080,7 @@ struct Unlisted {
     bool none;
     __device__ __forceinline__ Unlisted(const DistillArgs& a, const RowGradient& q, float scale) {
         none = q.empty() || scale == 0.f;
-        const bool far = fabsf(q.m) > BIG;
+        const bool far = !ref_near(reference(q.m, a.c));
         sub = far ? q.m : 0.f;
         R = far || none ? 0.f : reference(q.m, a.c);
         f = none ? 0.f : scale * q.f;

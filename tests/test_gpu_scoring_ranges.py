@@ -1,0 +1,188 @@
+"""Class scoring and distillation of rows of any magnitude, on the GPU against float64 (oracle/score_oracle.py): rows masked with ordinary
+large values (-1e4 ... -1e30), forced tokens, large common offsets, rows that hold NaN.
+
+Softmax does not know a common offset, so the bounds here know none either: everything is relative to distances from the row's maximum m.
+u = 2^-24 (half a step of float32, relative).  z - m, the rounding of T to float32, of 1 / T (or log2 e / T) and the product cost 4 u of
+the distance |y - m|: 6 u is allowed.  A sum of C exponentials adds at most ~C / 64 terms one after the other per thread, each off by a few
+u (the hardware's 2^x: 2 u): `terms` = 16 + C / 64 + 4 log2 C in units of u.  The log-sum-exp itself is of the row's magnitude: 4 u of it.
+Results of fewer bits add half a step of their type."""
+import math
+
+import pytest
+import torch
+
+from oracle import score_oracle as so
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+DT = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+NEG = float("-inf")
+NAN = float("nan")
+
+
+@pytest.fixture(scope="module")
+def eng():
+    from mica_amd.engine import Engine
+    e = Engine(0, max_batch=1, tile_size=4)
+    yield e
+    e.close()
+
+
+def _rng(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _log2c(c):
+    return math.log2(c) + 4.0
+
+
+def _terms(c):
+    return 16 + c / 64 + 4 * _log2c(c)
+
+
+def _herr(c):
+    """of the entropy: the same terms weighted once more with |log p|"""
+    return U * (32 + c / 32 + 6 * _log2c(c) ** 2)
+
+
+def _finite(t):
+    return torch.nan_to_num(t, nan=0.0, posinf=0.0, neginf=0.0)
+
+
+def _near(got, want, tol, what=""):
+    """got against want, infinities and NaN at the same places; tol per element"""
+    got = got.detach().cpu().double()
+    want = want.double()
+    assert got.shape == want.shape
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), what
+    inf = torch.isinf(want)
+    assert torch.equal(torch.isinf(got), inf) and torch.equal(got[inf], want[inf]), what
+    ok = ~(inf | torch.isnan(want))
+    tol = torch.as_tensor(tol, dtype=torch.float64).expand(want.shape)
+    over = ((got - want).abs() / tol)[ok]
+    worst = float(over.max()) if bool(ok.any()) else 0.0
+    assert worst <= 1.0, f"{what}: {worst} times the bound"
+
+
+def _half_step(dtype, want):
+    t = DT[dtype]
+    if t == torch.float32:
+        return U * want.abs() + 1e-37
+    return torch.finfo(t).eps / 2 * want.abs() + (torch.finfo(t).smallest_normal * torch.finfo(t).eps)
+
+
+def _values(dtype):
+    if dtype == "f16":
+        return [-1e4, -65504.0]
+    return [-1e4, -65504.0, -1e6, -1e7, -1e9, -1e10, -1e12, -1e20, -1e30]
+
+
+def _rows(classes, value, dtype, seed):
+    """rows that hold `value` in different places, and one that does not"""
+    g = _rng(seed)
+    z = torch.randn((8, classes), generator=g) * 3.0
+    half = classes // 2
+    z[0] = value
+    z[1, :half] = value                                      # whole threads see nothing but the value first
+    keep = z[2, classes - 1].clone()
+    z[2] = value
+    z[2, classes - 1] = keep
+    z[3, torch.rand((classes,), generator=g) < 0.6] = value
+    z[4, half] = -value                                      # a forced class
+    z[5] = -value
+    z[6, :half] = value
+    z[6, half:] = value * (1.0 - 2.0 ** -7)
+    return z.to(DT[dtype])
+
+
+def _tokens(classes):
+    return torch.tensor([classes - 1, 0, classes - 1, classes // 3, classes // 2, 1, classes - 1, -100])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("classes", [21, 65, 300, 5000, 70001])
+@pytest.mark.parametrize("temperature", [0.1, 0.7, 1.0, 2.0])
+def test_scores_of_rows_of_any_magnitude(eng, dtype, classes, temperature):
+    tok = _tokens(classes)
+    for value in _values(dtype):
+        z = _rows(classes, value, dtype, classes)
+        r = eng.token_logprobs(z.cuda(), tok.cuda(), top=5, temperature=temperature)
+        w = so.score(z, tok, 5, temperature)
+        what = f"value {value}"
+        _near(r.lse, w["lse"], U * (_terms(classes) + 4 * w["lse"].abs()), what)
+        _near(r.logprob, w["logprob"], U * (_terms(classes) + 6 * w["logprob"].abs()), what)
+        _near(r.entropy, w["entropy"], _herr(classes), what)
+        assert torch.equal(r.top_index.cpu().long(), w["top_index"]), what
+        _near(r.top_logprob, w["top_logprob"], U * (_terms(classes) + 6 * w["top_logprob"].abs()), what)
+
+
+def _check_distill(eng, z, idx, val, dtype, temperature, tail, weight, what=""):
+    """loss, gradient and the one-call step, bounds by distances alone"""
+    want, wgrad, p = so.distill(z, idx, val, temperature, tail)
+    C = z.shape[-1]
+    y = z.double() / temperature
+    logq = so.log_softmax(y)[0]
+    listed = torch.zeros(y.shape[:-1] + (C + 1,), dtype=torch.bool).scatter_(-1, torch.where(idx < 0, C, idx).long(), True)[..., :C]
+    free = torch.where(listed, torch.full_like(y, NEG), y)
+    mrest = free.amax(-1, keepdim=True)
+    # of listed classes to the row's maximum, of the others to theirs; what has no probability has no error
+    dist = torch.where(listed, (y - y.amax(-1, keepdim=True)).abs(), (y - torch.where(torch.isinf(mrest), torch.zeros_like(mrest), mrest)).abs())
+    shown = torch.where(torch.exp(-dist) > 0, dist, torch.zeros_like(dist))
+    lqr = torch.logsumexp(torch.where(listed, torch.full_like(y, NEG), logq), -1)
+    lq = torch.maximum(_finite(p["lq"]).abs().amax(-1), torch.where(p["rest"] > 0, _finite(lqr).abs(), torch.zeros_like(lqr)))
+    t = torch.where(idx < 0, torch.full_like(val, NEG), val).double()
+    tmax = torch.zeros_like(t[..., :1]) if tail else t.amax(-1, keepdim=True)
+    lt = _finite(t - tmax).abs().amax(-1, keepdim=True)
+    mass = p["mass"][..., 0].clamp(min=1.0)
+    loss_tol = temperature ** 2 * U * (_terms(C) + 6 * lq + 4 * lt[..., 0]) * mass + 2 * U * _finite(want).abs() + 1e-37
+    d = [x.cuda() for x in (z, idx, val)]
+    loss, aux = eng.distill_loss(*d, temperature=temperature, tail=tail)
+    _near(loss, want, loss_tol, what)
+    w = weight.double()[..., None]
+    both = p["q"] * p["mass"] + p["share"] * p["rest"][..., None]
+    tol = temperature * w.abs() * U * ((16 + 6 * shown + _terms(C)) * both + (16 + 6 * lt) * p["target"]) + _half_step(dtype, wgrad * w) + 1e-37
+    got = eng.distill_backward(*d, aux, weight.cuda(), temperature=temperature, tail=tail)
+    _near(got, wgrad * w, tol, what)
+    sl, sg = eng.distill_step(*d, temperature=temperature, tail=tail, weight=weight.cuda())
+    _near(sl, want * weight.double(), loss_tol * weight.double().abs() + 2 * U * _finite(want).abs() * weight.double().abs(), what)
+    _near(sg, wgrad * w, tol, what)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("classes", [21, 65, 300, 5000, 70001])
+@pytest.mark.parametrize("tail", [False])
+def test_distillation_of_rows_of_any_magnitude(eng, dtype, classes, tail):
+    g = _rng(classes)
+    idx = torch.stack([torch.randperm(classes, generator=g)[:6] for _ in range(8)]).int()
+    idx[:, 5] = -1
+    idx[2, 0] = classes - 1
+    idx[4, 0] = classes // 2
+    for r in range(8):                                       # distinct again
+        seen = set()
+        for k in range(5):
+            while int(idx[r, k]) in seen:
+                idx[r, k] = (int(idx[r, k]) + 1) % classes
+            seen.add(int(idx[r, k]))
+    val = torch.log(torch.tensor([0.4, 0.3, 0.1, 0.05, 0.02, 0.9])).repeat(8, 1)
+    weight = torch.rand((8,), generator=g) + 0.5
+    for value in _values(dtype):
+        z = _rows(classes, value, dtype, classes)
+        for temperature in (0.1, 1.0, 2.0):
+            _check_distill(eng, z, idx, val, dtype, temperature, tail, weight, f"value {value}, T {temperature}")
+
+
+def test_a_call_of_few_rows_and_many_agree_on_masked_rows(eng):
+    """cut into segments (each with a maximum of its own, some of masked classes only) or whole"""
+    classes = 40000
+    for value in (-1e9, -1e10, -1e20):
+        z = torch.full((300, classes), value)
+        z[:, 30000:30100] = torch.randn((300, 100), generator=_rng(1))
+        z[1] = value
+        a = eng.token_logprobs(z[:4].cuda(), torch.arange(4).cuda() + 30000, top=9)
+        b = eng.token_logprobs(z.cuda(), torch.arange(300).cuda() % 100 + 30000, top=9)
+        assert torch.equal(a.top_index, b.top_index[:4])
+        for x, y in zip(a, b):
+            assert float((x - y[:4]).abs().nan_to_num().max()) <= U * 2 * _terms(classes) + 4 * U * float(y[:4].abs().max()) and bool(torch.isfinite(x).all())
+        w = so.score(z[:4], torch.arange(4) + 30000, 9)
+        _near(a.logprob, w["logprob"], U * (_terms(classes) + 6 * w["logprob"].abs()))
