@@ -970,7 +970,9 @@ __device__ __forceinline__ RowScalars row_scalars(const DistillArgs& a, const Li
             o.M = fmaxf(m, l.zmax);
             const double u = ((double)l.zmax - m) * a.inv_t + l.log_sl - log_m;      // log of (listed sum / rest sum)
             o.log_q_rest = -(u > 700.0 ? u : log1p(exp(u)));
-            o.log_s = ((double)m - o.M) * a.inv_t + log_m - o.log_q_rest;
+            // relative to M, as two parts of which the larger one is about 1 or more: through u, a listed class 1e12 above would swallow it
+            const double r = ((double)m - o.M) * a.inv_t + log_m, t = ((double)l.zmax - o.M) * a.inv_t + l.log_sl;
+            o.log_s = fmax(r, t) + log1p(exp(-fabs(r - t)));
         }
         factor = o.mass * exp(o.log_q_rest) - o.rest;
     }

@@ -87,10 +87,11 @@ def distill(z, index, value, temperature=1.0, tail=False):
     at = index.long().clamp(min=0)
     lq = torch.gather(logq, -1, at)
     loss = torch.where(p == 0, torch.zeros_like(p), p * (logp - lq)).sum(-1)
-    free = torch.where(listed, torch.full_like(logq, NEG), logq)
+    free = torch.where(listed, torch.full_like(y, NEG), y)         # of y, not of logq: beside a class at 1e12 logq has lost their distances
     some = (free > NEG).any(-1)
     rest = torch.where(some, rest, torch.zeros_like(rest))
-    lfree, lqr = log_softmax(free)
+    lfree = log_softmax(free)[0]
+    lqr = (free.amax(-1) - y.amax(-1)) - lfree.amax(-1) + logq.amax(-1)      # maxima apart, log sums apart: a huge maximum would swallow the sum
     loss = loss + torch.where(rest > 0, rest * (torch.log(rest.clamp(min=1e-300)) - torch.where(rest > 0, lqr, torch.zeros_like(lqr))), torch.zeros_like(rest))
     mass = (p.sum(-1) + rest).unsqueeze(-1)
     grad = mass * q - target - torch.where((rest > 0).unsqueeze(-1) & ~listed, rest.unsqueeze(-1) * torch.exp(lfree), torch.zeros_like(q))
