@@ -14,8 +14,8 @@
  *     data_ptr()); h_* is HOST memory.  `stream` is a hipStream_t passed as void* (NULL = default).
  *   - one mica_ctx per GPU; a ctx is not thread-safe, different ctxs are independent.
  *   - kernels are launched on `stream`.  Which calls return before the device work is done is stated per function:
- *       asynchronous (enqueue and return): mica_gather_tiles(_u8), mica_stitch_tiles, mica_postprocess, mica_token_logprobs(_backward),
- *       mica_distill_loss / _backward / _step (these five can be captured into a graph);
+ *       asynchronous (enqueue and return): mica_gather_tiles(_u8), mica_stitch_tiles, mica_postprocess, mica_token_logprobs(_aux, _backward),
+ *       mica_distill_loss / _backward / _step (these six can be captured into a graph);
  *       SYNCHRONISE `stream` before returning: mica_forward_logits / _tiles / _records (they read back the per-tile |AF3| sums that
  *       pick the branch of models/model.py:56-63 and the per-tile range flags of the split-f16 encoding, and may repeat a tile, see
  *       mica_get_last_forward_scale), mica_finalize_weights, mica_normalise_map*, mica_zoom_cubic*, mica_rasterise_atoms, the point-list
@@ -52,7 +52,8 @@ typedef struct mica_ctx mica_ctx;
 #define MICA_AF_ALWAYS 3    /* no test: every tile takes the AF3 branch - for a caller that cut one batch into several calls and
                                evaluated the batch-wide test itself (mica_amd/engine.py does for batches beyond max_batch)      */
 
-int mica_abi_version(void);   /* 4 (3: mica_get_last_forward_input_runs, mica_get_last_forward_af_tiles; 4: mica_token_logprobs*, mica_distill_*); bumped with every export or struct change */
+int mica_abi_version(void);   /* 5 (3: mica_get_last_forward_input_runs, mica_get_last_forward_af_tiles; 4: mica_token_logprobs*, mica_distill_*;
+                                 5: mica_token_logprobs_aux, mica_token_logprobs_backward reads its d_aux); bumped with every export or struct change */
 
 /* ---- context ---------------------------------------------------------------------------- */
 /* Allocates the activation workspace for up to max_batch tiles of tile_size^3 voxels in flight (about 4.6 GB per 64^3 tile).
@@ -267,11 +268,17 @@ int64_t mica_token_logprobs_ws(const mica_logits* z, int top);      /* bytes; < 
 int mica_token_logprobs(mica_ctx* ctx, const mica_logits* z, const void* d_tokens, int token_bytes, int64_t ignore_index, float temperature,
                         int top, float* d_logprob, float* d_entropy, float* d_lse, float* d_top_logprob, int32_t* d_top_index,
                         void* d_ws, int64_t ws_bytes, void* stream);
+/* The same, and d_aux f32[2][rows] for the gradient: every row's maximum m and sum_v e^{(z_v - m) / T}, kept apart because a float32 log sum of
+ * a row of large magnitude has lost the sum (neither written nor read for classes <= 64; nullable there).  d_ws may be NULL: no row is cut
+ * into segments then, and a row's results do not depend on the number of rows (few long rows take longer).                          */
+int mica_token_logprobs_aux(mica_ctx* ctx, const mica_logits* z, const void* d_tokens, int token_bytes, int64_t ignore_index, float temperature,
+                            int top, float* d_logprob, float* d_entropy, float* d_lse, float* d_aux, float* d_top_logprob, int32_t* d_top_index,
+                            void* d_ws, int64_t ws_bytes, void* stream);
 /* d_grad (the logits' type, laid out as class_last says) = gradient of sum_n g_logprob logprob + g_entropy entropy + g_lse lse; each of
- * the three upstream gradients f32[rows] is nullable.  d_lse, d_entropy: what the forward call wrote.  0 in a row without a finite
- * class; a token out of range makes its row's gradient NaN.                                                                       */
+ * the three upstream gradients f32[rows] is nullable.  d_aux, d_entropy: what mica_token_logprobs_aux wrote for the same logits and
+ * temperature.  0 in a row without a finite class; a token out of range makes its row's gradient NaN.                              */
 int mica_token_logprobs_backward(mica_ctx* ctx, const mica_logits* z, const void* d_tokens, int token_bytes, int64_t ignore_index,
-                                 float temperature, const float* d_lse, const float* d_entropy, const float* d_g_logprob,
+                                 float temperature, const float* d_aux, const float* d_entropy, const float* d_g_logprob,
                                  const float* d_g_entropy, const float* d_g_lse, void* d_grad, void* stream);
 /* A teacher's K (1 .. 256) alternatives per row, C-contiguous [outer][inner][K] or [outer][K][inner] as the logits' class_last says:
  * d_index (4- or 8-byte integers, negative = unused entry), d_value = their log probabilities at the loss's temperature.  A class named

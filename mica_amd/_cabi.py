@@ -8,7 +8,7 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libmica_hip.so")
 
-ABI_VERSION = 4          # mica_abi_version() of the library these signatures describe (bumped whenever an export or a struct changes)
+ABI_VERSION = 5          # mica_abi_version() of the library these signatures describe (bumped whenever an export or a struct changes)
 MICA_OK = 0
 MICA_ERR_ARG, MICA_ERR_HIP, MICA_ERR_STATE, MICA_ERR_RANGE = -1, -2, -3, -4
 AF_NONE, AF_PER_TILE, AF_BATCH, AF_ALWAYS = 0, 1, 2, 3
@@ -69,6 +69,7 @@ SIGNATURES = {
     "mica_neighbour_matrix_np": (_I, [_P, _P, _L, _P, _L, _L, _L, _I, _P, _P, _P]),
     "mica_token_logprobs_ws": (_L, [_ZP, _I]),
     "mica_token_logprobs": (_I, [_P, _ZP, _P, _I, _L, _F, _I, _P, _P, _P, _P, _P, _P, _L, _P]),
+    "mica_token_logprobs_aux": (_I, [_P, _ZP, _P, _I, _L, _F, _I, _P, _P, _P, _P, _P, _P, _P, _L, _P]),
     "mica_token_logprobs_backward": (_I, [_P, _ZP, _P, _I, _L, _F, _P, _P, _P, _P, _P, _P, _P]),
     "mica_distill_ws": (_L, [_ZP, _I]),
     "mica_distill_loss": (_I, [_P, _ZP, _TP, _F, _P, _P, _P, _L, _P]),

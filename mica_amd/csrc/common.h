@@ -287,8 +287,8 @@ SegPlan score_segments(const LogitsView& v, int64_t rows);
 int64_t score_ws_bytes(const LogitsView& v, int64_t rows, int top);
 int64_t distill_ws_bytes(const LogitsView& v, int64_t rows, bool step);
 void launch_score(const LogitsView& v, int64_t rows, const void* tokens, int token_bytes, int64_t ignore, float temperature, int top, float* logprob,
-                  float* entropy, float* lse, float* top_logprob, int* top_index, void* ws, hipStream_t st);
-void launch_score_grad(const LogitsView& v, int64_t rows, const void* tokens, int token_bytes, int64_t ignore, float temperature, const float* lse,
+                  float* entropy, float* lse, float* aux, float* top_logprob, int* top_index, void* ws, hipStream_t st);
+void launch_score_grad(const LogitsView& v, int64_t rows, const void* tokens, int token_bytes, int64_t ignore, float temperature, const float* aux,
                        const float* entropy, const float* g_logprob, const float* g_entropy, const float* g_lse, void* grad, hipStream_t st);
 void launch_distill_loss(const LogitsView& v, int64_t rows, const DistillList& d, float temperature, float* loss, float* aux, void* ws, hipStream_t st);
 void launch_distill_grad(const LogitsView& v, int64_t rows, const DistillList& d, float temperature, const float* aux, const float* g_loss, void* grad,

@@ -631,7 +631,7 @@ static int forward_checked(mica_ctx* c, const float* d_map, const float* d_af, i
 // =================================================================================================
 extern "C" {
 
-int mica_abi_version(void) { return 4; }
+int mica_abi_version(void) { return 5; }
 
 const char* mica_last_error(const mica_ctx* ctx) { return ctx ? ctx->err.c_str() : g_create_err.c_str(); }
 
@@ -1453,7 +1453,7 @@ bool bad_temperature(float t) { return !(t >= 1e-4f && t <= 1e4f); }
 
 #define SCORE_REFUSE(c, name, why)                                  \
     do {                                                            \
-        (c)->err = std::string(name ": ") + (why);                  \
+        (c)->err = std::string(name) + ": " + (why);                \
         return MICA_ERR_ARG;                                        \
     } while (0)
 
@@ -1464,31 +1464,48 @@ int64_t mica_token_logprobs_ws(const mica_logits* z, int top) {
     return rows ? score_ws_bytes(v, rows, top) : 0;
 }
 
-int mica_token_logprobs(mica_ctx* c, const mica_logits* z, const void* d_tokens, int token_bytes, int64_t ignore_index, float temperature, int top,
-                        float* d_logprob, float* d_entropy, float* d_lse, float* d_top_logprob, int32_t* d_top_index, void* d_ws, int64_t ws_bytes,
-                        void* stream) {
-    if (!c) return MICA_ERR_ARG;
+// d_aux: null from mica_token_logprobs; whole: rows are not cut, whatever their number, and no workspace is needed
+static int score_call(mica_ctx* c, const mica_logits* z, const void* d_tokens, int token_bytes, int64_t ignore_index, float temperature, int top,
+                      float* d_logprob, float* d_entropy, float* d_lse, float* d_aux, bool whole, float* d_top_logprob, int32_t* d_top_index, void* d_ws,
+                      int64_t ws_bytes, void* stream, const char* name) {
     LogitsView v;
     int64_t rows = 0;
-    if (const char* why = logits_view(z, v, rows)) SCORE_REFUSE(c, "mica_token_logprobs", why);
-    if (bad_temperature(temperature)) SCORE_REFUSE(c, "mica_token_logprobs", "temperature must be in [1e-4, 1e4]");
-    if (top < 0 || top > 64 || top > v.classes) SCORE_REFUSE(c, "mica_token_logprobs", "top must be in [0, min(64, classes)]");
+    if (const char* why = logits_view(z, v, rows)) SCORE_REFUSE(c, name, why);
+    if (bad_temperature(temperature)) SCORE_REFUSE(c, name, "temperature must be in [1e-4, 1e4]");
+    if (top < 0 || top > 64 || top > v.classes) SCORE_REFUSE(c, name, "top must be in [0, min(64, classes)]");
     if (!rows) return MICA_OK;
     if (!d_entropy || !d_lse || (d_tokens == nullptr) != (d_logprob == nullptr) || (d_tokens && token_bytes != 4 && token_bytes != 8) ||
         (top > 0 && (!d_top_logprob || !d_top_index)))
-        SCORE_REFUSE(c, "mica_token_logprobs", "null pointer or token size");
-    const int64_t need = score_ws_bytes(v, rows, top);
-    if (need > 0 && (!d_ws || ws_bytes < need || ((uintptr_t)d_ws & 15))) SCORE_REFUSE(c, "mica_token_logprobs", "workspace too small or misaligned");
+        SCORE_REFUSE(c, name, "null pointer or token size");
+    const int64_t need = whole ? 0 : score_ws_bytes(v, rows, top);
+    if (need > 0 && (!d_ws || ws_bytes < need || ((uintptr_t)d_ws & 15))) SCORE_REFUSE(c, name, "workspace too small or misaligned");
     DeviceGuard guard;
     MICA_ENTER(c);
-    launch_score(v, rows, d_tokens, token_bytes, ignore_index, temperature, top, d_logprob, d_entropy, d_lse, d_top_logprob, d_top_index, d_ws,
-                 (hipStream_t)stream);
+    launch_score(v, rows, d_tokens, token_bytes, ignore_index, temperature, top, d_logprob, d_entropy, d_lse, d_aux, d_top_logprob, d_top_index,
+                 need > 0 ? d_ws : nullptr, (hipStream_t)stream);
     CHECK_LAUNCHES(c);
     return MICA_OK;
 }
 
+int mica_token_logprobs(mica_ctx* c, const mica_logits* z, const void* d_tokens, int token_bytes, int64_t ignore_index, float temperature, int top,
+                        float* d_logprob, float* d_entropy, float* d_lse, float* d_top_logprob, int32_t* d_top_index, void* d_ws, int64_t ws_bytes,
+                        void* stream) {
+    if (!c) return MICA_ERR_ARG;
+    return score_call(c, z, d_tokens, token_bytes, ignore_index, temperature, top, d_logprob, d_entropy, d_lse, nullptr, false, d_top_logprob, d_top_index,
+                      d_ws, ws_bytes, stream, "mica_token_logprobs");
+}
+
+int mica_token_logprobs_aux(mica_ctx* c, const mica_logits* z, const void* d_tokens, int token_bytes, int64_t ignore_index, float temperature, int top,
+                            float* d_logprob, float* d_entropy, float* d_lse, float* d_aux, float* d_top_logprob, int32_t* d_top_index, void* d_ws,
+                            int64_t ws_bytes, void* stream) {
+    if (!c) return MICA_ERR_ARG;
+    if (!d_aux && z && z->classes > SCORE_COL_MAX && z->outer > 0 && z->inner > 0) SCORE_REFUSE(c, "mica_token_logprobs_aux", "null pointer");
+    return score_call(c, z, d_tokens, token_bytes, ignore_index, temperature, top, d_logprob, d_entropy, d_lse, d_aux, !d_ws, d_top_logprob, d_top_index, d_ws,
+                      ws_bytes, stream, "mica_token_logprobs_aux");
+}
+
 int mica_token_logprobs_backward(mica_ctx* c, const mica_logits* z, const void* d_tokens, int token_bytes, int64_t ignore_index, float temperature,
-                                 const float* d_lse, const float* d_entropy, const float* d_g_logprob, const float* d_g_entropy, const float* d_g_lse,
+                                 const float* d_aux, const float* d_entropy, const float* d_g_logprob, const float* d_g_entropy, const float* d_g_lse,
                                  void* d_grad, void* stream) {
     if (!c) return MICA_ERR_ARG;
     LogitsView v;
@@ -1496,11 +1513,11 @@ int mica_token_logprobs_backward(mica_ctx* c, const mica_logits* z, const void* 
     if (const char* why = logits_view(z, v, rows)) SCORE_REFUSE(c, "mica_token_logprobs_backward", why);
     if (bad_temperature(temperature)) SCORE_REFUSE(c, "mica_token_logprobs_backward", "temperature must be in [1e-4, 1e4]");
     if (!rows) return MICA_OK;
-    if (!d_lse || !d_entropy || !d_grad || (d_g_logprob && (!d_tokens || (token_bytes != 4 && token_bytes != 8))))
+    if ((!d_aux && !score_is_col(v)) || !d_entropy || !d_grad || (d_g_logprob && (!d_tokens || (token_bytes != 4 && token_bytes != 8))))
         SCORE_REFUSE(c, "mica_token_logprobs_backward", "null pointer or token size");
     DeviceGuard guard;
     MICA_ENTER(c);
-    launch_score_grad(v, rows, d_tokens, token_bytes, ignore_index, temperature, d_lse, d_entropy, d_g_logprob, d_g_entropy, d_g_lse, d_grad,
+    launch_score_grad(v, rows, d_tokens, token_bytes, ignore_index, temperature, d_aux, d_entropy, d_g_logprob, d_g_entropy, d_g_lse, d_grad,
                       (hipStream_t)stream);
     CHECK_LAUNCHES(c);
     return MICA_OK;

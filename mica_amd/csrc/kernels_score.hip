@@ -564,6 +564,8 @@ struct ScoreOut {
     int* top_index;
     int top;
     float c, inv_t;
+    float* aux;         // [2][rows], nullable: maximum and sum of e^{(z - maximum) / T}, for the gradient
+    int64_t rows;
 };
 // L: the type the row's scalars are combined in
 template <typename L> __device__ __forceinline__ float class_logprob(float z, float m, L log_s, float inv_t) {
@@ -578,6 +580,10 @@ __device__ __forceinline__ void write_row(const ScoreOut& o, const T* __restrict
     const L log2_s = sizeof(L) == 8 ? (L)log2((double)s) : (L)log2f(s);
     const float h = s == 0.f ? 0.f : (float)((L)LN2 * (log2_s - (L)w / (L)s));
     o.entropy[r] = h < 0.f ? 0.f : h;
+    if (o.aux) {
+        o.aux[r] = m;
+        o.aux[o.rows + r] = s * exp2_hw(-ref_residue(m, o.c));
+    }
     if (o.logprob) {
         const int64_t t = load_int(o.tokens, r, o.token_bytes);
         float lp;
@@ -703,42 +709,35 @@ __global__ __launch_bounds__(TOP ? JOIN : 64) void score_join_kernel(LogitsView 
 }
 
 // ---- gradient of the scores ------------------------------------------------------------------------------------------------------------
-// dz_v = (1/T) [ g_lp ([v = t] - p_v) + g_lse p_v - g_H p_v (log p_v + H) ]: one read, one write, no state but lse and H.  HBM-bound:
-// 4096 x 32000 bf16 89 us = 5.9 TB/s, above the rate of a copy because the forward pass left part of the logits in the Infinity Cache.
+// dz_v = (1/T) [ g_lp ([v = t] - p_v) + g_lse p_v - g_H p_v (log p_v + H) ]: one read, one write.  p = 2^d / S with d = (z - m) c, from the
+// row's maximum m and sum S apart: a float32 log sum of a row of large magnitude has lost log S (a row of -1e9: all of it).  Streamed rows
+// get both from the forward pass, the column kernel has the classes in registers and sums again.  HBM-bound: 4096 x 32000 bf16 92 us = 5.7
+// TB/s, above the rate of a copy because the forward pass left part of the logits in the Infinity Cache.
 struct ScoreGrad {
     const void* tokens;
     int token_bytes;
     int64_t ignore;
-    const float* lse;
+    const float* aux;
+    int64_t rows;
     const float* entropy;
     const float* g_logprob;
     const float* g_entropy;
     const float* g_lse;
     float c, inv_t;
 };
-constexpr float BIG = 1.0e30f;
 struct RowGrad {
-    float l2;           // lse in units of log 2
-    float a;            // coefficient of p
-    float b;            // coefficient of p log2 p
+    float m, c;
+    float a;            // coefficient of 2^d
+    float b;            // coefficient of 2^d d
     float at_token;     // added at the token
     int64_t token;      // -1: none
     bool empty;
-    // |lse| > BIG (a row of the type's lowest values): lse is the maximum, float32 has lost the log of the sum; the classes that reach it
-    // share the row, one e^{-H} each, and every other one lies beyond any exponent
-    bool far;
-    float lse, inv_t, far_p, far_log2p;
 };
-__device__ __forceinline__ RowGrad row_grad(const ScoreGrad& o, int64_t classes, int64_t r) {
+__device__ __forceinline__ RowGrad row_grad(const ScoreGrad& o, int64_t classes, int64_t r, float m, float s) {
     RowGrad g;
-    const float lse = o.lse[r];
-    g.empty = lse == -INFINITY;
-    g.far = fabsf(lse) > BIG && !g.empty;
-    g.lse = lse;
-    g.inv_t = o.inv_t;
-    g.far_log2p = -o.entropy[r] * LOG2E;
-    g.far_p = exp2_hw(g.far_log2p);
-    g.l2 = lse * LOG2E;
+    g.empty = m == -INFINITY && s == 0.f;
+    g.m = m;
+    g.c = o.c;
     float glp = 0.f;
     g.token = -1;
     if (o.g_logprob) {
@@ -750,22 +749,15 @@ __device__ __forceinline__ RowGrad row_grad(const ScoreGrad& o, int64_t classes,
         }
     }
     const float ge = o.g_entropy ? o.g_entropy[r] : 0.f, gl = o.g_lse ? o.g_lse[r] : 0.f;
-    g.a = (gl - glp - (ge != 0.f ? ge * o.entropy[r] : 0.f)) * o.inv_t;
-    g.b = -ge * (float)LN2 * o.inv_t;
+    const float scale = o.inv_t / s;                        // log p + H = d log 2 + (H - log S)
+    g.a = (gl - glp - (ge != 0.f ? ge * (o.entropy[r] - logf(s)) : 0.f)) * scale;
+    g.b = -ge * (float)LN2 * scale;
     g.at_token = g.empty ? 0.f : glp * o.inv_t;
     return g;
 }
-template <bool FAR> __device__ __forceinline__ float grad_value(const RowGrad& g, float z, float c) {
-    float x, p;
-    if (FAR) {
-        const bool reaches = z != -INFINITY && finite((float)((double)z * g.inv_t)) == g.lse;
-        x = reaches ? g.far_log2p : NEG_BIG;
-        p = reaches ? g.far_p : 0.f;
-    } else {
-        x = fmaf(z, c, -g.l2);
-        p = exp2_hw(x);
-    }
-    return g.empty ? 0.f : p * fmaf(g.b, fmaxf(x, NEG_BIG), g.a);
+__device__ __forceinline__ float grad_value(const RowGrad& g, float z) {
+    const float d = (z - g.m) * g.c;
+    return g.empty ? 0.f : exp2_hw(d) * fmaf(g.b, fmaxf(d, NEG_BIG), g.a);
 }
 
 // what a block of the gradient kernels covers: G threads x UNROLL vectors of one row
@@ -802,15 +794,9 @@ __global__ __launch_bounds__(256) void score_grad_row_kernel(LogitsView v, int64
     if (item >= rows * chunks) return;
     const int64_t r = chunks == 1 ? item : item / chunks;
     const int first = chunks == 1 ? 0 : (int)(item % chunks) * CHUNK;
-    const RowGrad g = row_grad(o, v.classes, r);
+    const RowGrad g = row_grad(o, v.classes, r, o.aux[r], o.aux[o.rows + r]);
     const T* z = static_cast<const T*>(v.p) + row_start(v, row_pos(v, r));
-    const auto chunk = [&](auto far) {
-        map_chunk<T, G, ONCE>(z, grad + r * v.classes, first, v.classes, tid, [&](float x, int64_t at) {
-            return grad_value<decltype(far)::value>(g, x, o.c) + (at == g.token ? g.at_token : 0.f);
-        });
-    };
-    if (__builtin_expect(g.far, 0)) chunk(std::true_type());
-    else chunk(std::false_type());
+    map_chunk<T, G, ONCE>(z, grad + r * v.classes, first, v.classes, tid, [&](float x, int64_t at) { return grad_value(g, x) + (at == g.token ? g.at_token : 0.f); });
 }
 
 // ---- distillation ------------------------------------------------------------------------------------------------------------------------
@@ -1239,12 +1225,16 @@ __global__ __launch_bounds__(256) void score_grad_col_kernel(LogitsView v, int64
     const RowPos p = row_pos(v, r);
     float z[CM];
     load_classes(z, static_cast<const T*>(v.p) + row_start(v, p), v.sc, classes);
-    const RowGrad g = row_grad(o, classes, r);
+    const float m = max_of(z), ref = m == -INFINITY ? 0.f : m;
+    float s = 0.f;
+#pragma unroll
+    for (int c = 0; c < CM; ++c) s += exp2_hw((z[c] - ref) * o.c);
+    const RowGrad g = row_grad(o, classes, r, m, s);
     T* out = grad + grad_start(v, p, r);
     const int64_t step = v.class_last ? 1 : v.inner;
 #pragma unroll
     for (int c = 0; c < CM; ++c)
-        if (c < classes) out[c * step] = from_f32<T>((g.far ? grad_value<true>(g, z[c], o.c) : grad_value<false>(g, z[c], o.c)) + (c == g.token ? g.at_token : 0.f));
+        if (c < classes) out[c * step] = from_f32<T>(grad_value(g, z[c]) + (c == g.token ? g.at_token : 0.f));
 }
 
 // Loss (a.loss) and / or gradient (grad) of a row; the gradient's scale: weight or the upstream gradient.  In float32, as a few classes
@@ -1418,8 +1408,9 @@ int64_t score_ws_bytes(const LogitsView& v, int64_t rows, int top) {
 }
 
 void launch_score(const LogitsView& v, int64_t rows, const void* tokens, int token_bytes, int64_t ignore, float temperature, int top,
-                  float* logprob, float* entropy, float* lse, float* top_logprob, int* top_index, void* ws, hipStream_t st) {
-    ScoreOut o{tokens, token_bytes, ignore, logprob, entropy, lse, top_logprob, top_index, top, LOG2E / temperature, 1.0f / temperature};
+                  float* logprob, float* entropy, float* lse, float* aux, float* top_logprob, int* top_index, void* ws, hipStream_t st) {
+    ScoreOut o{tokens, token_bytes, ignore, logprob, entropy, lse, top_logprob, top_index, top, LOG2E / temperature, 1.0f / temperature,
+               score_is_col(v) ? nullptr : aux, rows};
     by_dtype(v.dtype, [&](auto* tp) {
         using T = std::remove_pointer_t<decltype(tp)>;
         if (score_is_col(v)) {
@@ -1428,7 +1419,7 @@ void launch_score(const LogitsView& v, int64_t rows, const void* tokens, int tok
             });
             return;
         }
-        const SegPlan s = score_segments(v, rows);
+        const SegPlan s = ws ? score_segments(v, rows) : SegPlan{1, (int)v.classes};      // without a workspace every row is whole
         Partial* part = static_cast<Partial*>(ws);
         u64* part_top = reinterpret_cast<u64*>(part + rows * s.n);
         const int64_t items = rows * s.n;
@@ -1444,9 +1435,9 @@ void launch_score(const LogitsView& v, int64_t rows, const void* tokens, int tok
     });
 }
 
-void launch_score_grad(const LogitsView& v, int64_t rows, const void* tokens, int token_bytes, int64_t ignore, float temperature, const float* lse,
+void launch_score_grad(const LogitsView& v, int64_t rows, const void* tokens, int token_bytes, int64_t ignore, float temperature, const float* aux,
                        const float* entropy, const float* g_logprob, const float* g_entropy, const float* g_lse, void* grad, hipStream_t st) {
-    ScoreGrad o{tokens, token_bytes, ignore, lse, entropy, g_logprob, g_entropy, g_lse, LOG2E / temperature, 1.0f / temperature};
+    ScoreGrad o{tokens, token_bytes, ignore, aux, rows, entropy, g_logprob, g_entropy, g_lse, LOG2E / temperature, 1.0f / temperature};
     by_dtype(v.dtype, [&](auto* tp) {
         using T = std::remove_pointer_t<decltype(tp)>;
         T* out = static_cast<T*>(grad);

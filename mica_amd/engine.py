@@ -396,19 +396,21 @@ class Engine:
         return torch.empty((nbytes,), dtype=torch.uint8, device=self.device) if nbytes else None
 
     def token_logprobs(self, logits: torch.Tensor, tokens: torch.Tensor | None = None, top: int = 0, dim: int = -1, temperature: float = 1.0,
-                       ignore_index: int = -100, view=None):
+                       ignore_index: int = -100, view=None, aux=None):
         """Scores of the distributions softmax(logits / temperature) along `dim` -> scoring.TokenScores:
         logprob (of `tokens`, integers of the logits' shape without `dim`; ignore_index: 0, any other value outside [0, classes): NaN),
         entropy and lse (log sum exp), all float32; top_logprob float32 / top_index int32, the `top` (<= 64) most probable classes in
         order, ties to the lowest class.  Logits float32, bfloat16 or float16 of any strides.  A row whose classes are all -inf: log
         probabilities and lse -inf, entropy 0 (any other row's lse is kept within float32).  Asynchronous; the results have no autograd
-        history (scoring.token_logprobs has)."""
+        history (scoring.token_logprobs has).  aux: of logits_view(logits, dim).score_aux(), written for token_logprobs_backward."""
         v = self.logits_view(logits, dim) if view is None else view
         temperature = scoring.check_temperature(temperature)
         top = int(top)
         if not 0 <= top <= min(scoring.MAX_TOP, v.classes):
             raise MicaHipError(f"top must be in [0, {min(scoring.MAX_TOP, v.classes)}], got {top}")
         dev, shape = self.device, v.rows_shape
+        if aux is not None:
+            self._check_score_aux(aux, v)
         logprob = topv = topi = None
         if tokens is not None:
             tokens = scoring.check_ints(tokens, "tokens", shape, dev).contiguous()
@@ -423,18 +425,27 @@ class Engine:
             z = C.byref(v.desc)
             nws = self.lib.mica_token_logprobs_ws(z, top)
             ws = self._workspace(nws)
-            r = self.lib.mica_token_logprobs(self._h, z, _addr(tokens), tokens.element_size() if tokens is not None else 0, int(ignore_index), temperature,
-                                             top, _addr(logprob), entropy.data_ptr(), lse.data_ptr(), _addr(topv), _addr(topi), _addr(ws), nws,
-                                             self._raw_stream())
-            self._check(r, "mica_token_logprobs")
+            given = (self._h, z, _addr(tokens), tokens.element_size() if tokens is not None else 0, int(ignore_index), temperature, top, _addr(logprob),
+                     entropy.data_ptr(), lse.data_ptr())
+            lists_ws = (_addr(topv), _addr(topi), _addr(ws), nws, self._raw_stream())
+            if aux is None:
+                self._check(self.lib.mica_token_logprobs(*given, *lists_ws), "mica_token_logprobs")
+            else:
+                self._check(self.lib.mica_token_logprobs_aux(*given, aux.data_ptr(), *lists_ws), "mica_token_logprobs_aux")
         if v.moved and top:
             topv, topi = v.give(topv), v.give(topi)
         return scoring.TokenScores(logprob, entropy, lse, topv, topi)
 
+    def _check_score_aux(self, aux, v):
+        if v.classes <= scoring.COL_MAX or not scoring.check_floats(aux, "aux", (2, v.rows), self.device).is_contiguous():
+            raise MicaHipError("aux: expected what score_aux() of this view returns")
+
     def token_logprobs_backward(self, logits, tokens, lse, entropy, g_logprob=None, g_entropy=None, g_lse=None, dim: int = -1,
-                                temperature: float = 1.0, ignore_index: int = -100, view=None) -> torch.Tensor:
+                                temperature: float = 1.0, ignore_index: int = -100, view=None, aux=None) -> torch.Tensor:
         """Gradient, in the logits' type and shape, of (g_logprob logprob + g_entropy entropy + g_lse lse).sum(); lse and entropy are
-        token_logprobs' results for the same logits and temperature; each upstream gradient may be None."""
+        token_logprobs' results for the same logits and temperature; each upstream gradient may be None.  aux: what token_logprobs wrote
+        there; without it the rows' maxima and sums are taken from the logits once more (they cannot be had back from lse, whose rounding
+        is as large as log C in rows of large magnitude)."""
         v = self.logits_view(logits, dim) if view is None else view
         temperature = scoring.check_temperature(temperature)
         dev, shape = self.device, v.rows_shape
@@ -449,10 +460,18 @@ class Engine:
             tokens = scoring.check_ints(tokens, "tokens", shape, dev).contiguous()
         else:
             tokens = None
+        if aux is not None:
+            self._check_score_aux(aux, v)
         grad = torch.empty(v.with_axis(v.classes), dtype=v.dtype, device=dev)
         if v.rows:
-            r = self.lib.mica_token_logprobs_backward(self._h, C.byref(v.desc), _addr(tokens), tokens.element_size() if tokens is not None else 0,
-                                                      int(ignore_index), temperature, lse.data_ptr(), entropy.data_ptr(), _addr(g_logprob),
+            z = C.byref(v.desc)
+            if aux is None and v.classes > scoring.COL_MAX:
+                aux, unused = v.score_aux(), torch.empty((2, v.rows), dtype=torch.float32, device=dev)
+                r = self.lib.mica_token_logprobs_aux(self._h, z, None, 0, int(ignore_index), temperature, 0, None, unused[0].data_ptr(),
+                                                     unused[1].data_ptr(), aux.data_ptr(), None, None, None, 0, self._raw_stream())
+                self._check(r, "mica_token_logprobs_aux")
+            r = self.lib.mica_token_logprobs_backward(self._h, z, _addr(tokens), tokens.element_size() if tokens is not None else 0,
+                                                      int(ignore_index), temperature, _addr(aux), entropy.data_ptr(), _addr(g_logprob),
                                                       _addr(g_entropy), _addr(g_lse), grad.data_ptr(), self._raw_stream())
             self._check(r, "mica_token_logprobs_backward")
         return v.give(grad)

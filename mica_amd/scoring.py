@@ -102,6 +102,10 @@ class LogitsLayout:
             return None
         return (before or [(1, 0)])[0], after[0], False, sc
 
+    def score_aux(self):
+        """what token_logprobs hands to its backward pass: maximum and sum of every row; None for few classes, which a thread sums again"""
+        return torch.empty((2, self.rows), dtype=torch.float32, device=self.base.device) if self.classes > COL_MAX else None
+
     def with_axis(self, k):
         """shape with k entries at the class axis, as the library lays it out"""
         return self.rows_shape + (k,) if self.moved else self.shape[:self.dim] + (k,) + self.shape[self.dim + 1:]
@@ -154,10 +158,11 @@ class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, engine, tokens, top, dim, temperature, ignore_index):
         view = engine.logits_view(logits, dim)
-        r = engine.token_logprobs(logits, tokens, top, dim, temperature, ignore_index, view)
+        aux = view.score_aux()
+        r = engine.token_logprobs(logits, tokens, top, dim, temperature, ignore_index, view, aux)
         ctx.call = engine, view, temperature, ignore_index, dim
         # through save_for_backward, also what the view points into: torch refuses a backward pass over logits that were written since
-        ctx.save_for_backward(logits, r.lse, r.entropy, tokens)
+        ctx.save_for_backward(logits, r.lse, r.entropy, tokens, aux)
         if r.top_index is not None:
             ctx.mark_non_differentiable(r.top_logprob, r.top_index)
         ctx.set_materialize_grads(False)
@@ -168,9 +173,9 @@ class _TokenLogprobs(torch.autograd.Function):
     def backward(ctx, g_logprob, g_entropy, g_lse, *_):
         if g_logprob is None and g_entropy is None and g_lse is None:
             return (None,) * 7
-        logits, lse, entropy, tokens = ctx.saved_tensors
+        logits, lse, entropy, tokens, aux = ctx.saved_tensors
         engine, view, temperature, ignore_index, dim = ctx.call
-        return (engine.token_logprobs_backward(logits, tokens, lse, entropy, g_logprob, g_entropy, g_lse, dim, temperature, ignore_index, view),
+        return (engine.token_logprobs_backward(logits, tokens, lse, entropy, g_logprob, g_entropy, g_lse, dim, temperature, ignore_index, view, aux),
                 None, None, None, None, None, None)
 
 

@@ -225,3 +225,18 @@ def test_engine_answers_an_empty_tensor_without_a_call(eng):
     loss, aux = eng.distill_loss(torch.zeros(0, 300), torch.zeros(0, 3, dtype=torch.int32), torch.zeros(0, 3))
     assert loss.shape == (0,) and aux.shape == (4, 0)
     assert eng.distill_step(torch.zeros(0, 300), torch.zeros(0, 3, dtype=torch.int32), torch.zeros(0, 3))[1].shape == (0, 300)
+
+
+def test_the_gradients_maxima_and_sums_are_checked(eng):
+    """aux: one maximum and one sum per row of more than 64 classes, nothing for fewer"""
+    z, tok, row = torch.zeros(4, 100), torch.zeros(4, dtype=torch.int64), torch.zeros(4)
+    assert eng.logits_view(z, -1).score_aux().shape == (2, 4) and eng.logits_view(z[:, :64], -1).score_aux() is None
+    for aux in (torch.zeros(4), torch.zeros(4, 2), torch.zeros(2, 4, dtype=torch.float64), torch.zeros(4, 2).t(), torch.zeros(2, 4, device="meta"), 1.0):
+        with pytest.raises(MicaHipError):
+            eng.token_logprobs(z, tok, aux=aux)
+        with pytest.raises(MicaHipError):
+            eng.token_logprobs_backward(z, tok, row, row, g_logprob=row, aux=aux)
+    with pytest.raises(MicaHipError):
+        eng.token_logprobs(z[:, :64], tok, aux=torch.zeros(2, 4))
+    lib = _lib()
+    assert lib.mica_token_logprobs_aux(None, C.byref(_desc()), None, 0, -100, 1.0, 0, None, None, None, None, None, None, None, 0, None) == _cabi.MICA_ERR_ARG

@@ -186,3 +186,111 @@ def test_a_call_of_few_rows_and_many_agree_on_masked_rows(eng):
             assert float((x - y[:4]).abs().nan_to_num().max()) <= U * 2 * _terms(classes) + 4 * U * float(y[:4].abs().max()) and bool(torch.isfinite(x).all())
         w = so.score(z[:4], torch.arange(4) + 30000, 9)
         _near(a.logprob, w["logprob"], U * (_terms(classes) + 6 * w["logprob"].abs()))
+
+
+# ---- gradients of the scores -----------------------------------------------------------------------------------------------------------------
+
+def _grad_tol(z, dtype, want, gl, ge, gs, temperature):
+    """p is off by 6 u of its distance and `terms` u of the sum, log p likewise, the entropy by its own bound; the token's 1 - p rounds twice.
+    The hardware's 2^d is 0 below 2^-126, where p S < 2^-126: at most 2^-126 times what p is multiplied with is missing there."""
+    C = z.shape[-1]
+    w = so.score(z, temperature=temperature)
+    p = torch.exp(w["logp"])
+    y = z.double() / temperature
+    dist = torch.where(p > 0, (y - y.amax(-1, keepdim=True)).abs(), torch.zeros_like(y))
+    logp = torch.where(p > 0, w["logp"].abs(), torch.zeros_like(p))
+    a = (gl.double().abs() + gs.double().abs())[..., None]
+    e = ge.double().abs()[..., None]
+    H = w["entropy"][..., None]
+    own = U * (6 * dist + _terms(C))
+    tol = p * (own * (a + e * (logp + H)) + e * (_herr(C) + own + 4 * U * (logp + H))) / temperature
+    tol = tol + 2.0 ** -126 * (a + e * (logp + H)) / temperature
+    return tol + 4 * U * gl.double().abs()[..., None] / temperature * (want.abs() > 0) + _half_step(dtype, want) + 1e-37
+
+
+def _check_grad(eng, z, tok, dtype, gl, ge, gs, temperature, what=""):
+    """through autograd, and the engine's call on the forward results alone"""
+    from mica_amd import scoring
+    used = torch.where(tok == -100, torch.zeros_like(gl), gl)
+    want = so.score_grad(z, tok, gl, ge, gs, temperature)
+    tol = _grad_tol(z, dtype, want, used, ge, gs, temperature)
+    x = z.cuda().requires_grad_()
+    r = scoring.token_logprobs(eng, x, tok.cuda(), temperature=temperature)
+    got, = torch.autograd.grad([r.logprob, r.entropy, r.lse], [x], [gl.cuda(), ge.cuda(), gs.cuda()])
+    _near(got, want, tol, what)
+    alone = eng.token_logprobs_backward(z.cuda(), tok.cuda(), r.lse.detach(), r.entropy.detach(), gl.cuda(), ge.cuda(), gs.cuda(), temperature=temperature)
+    _near(alone, want, tol, what)
+    return got
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("classes", [7, 21, 65, 300, 5000, 70001])
+def test_score_gradients_of_rows_of_any_magnitude(eng, dtype, classes):
+    tok = _tokens(classes)
+    g = _rng(classes)
+    gl, ge, gs = (torch.randn((8,), generator=g) for _ in range(3))
+    for value in _values(dtype):
+        z = _rows(classes, value, dtype, classes)
+        for temperature in (0.1, 1.0, 2.0):
+            _check_grad(eng, z, tok, dtype, gl, ge, gs, temperature, f"value {value}, T {temperature}")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("classes", [21, 300, 70001])
+def test_score_gradients_of_rows_of_the_lowest_value_and_small_temperatures(eng, dtype, classes):
+    low = torch.finfo(DT[dtype]).min
+    z = torch.full((4, classes), low).to(DT[dtype])
+    z[1, ::2] = NEG
+    z[2] = NEG
+    z[2, [1, classes - 1]] = low
+    z[3] = 30.0
+    z[3, 2] = 30.0625 if dtype == "f32" else 30.125
+    tok = torch.tensor([1, 2, classes - 1, 2])
+    g = torch.tensor([1.0, -2.0, 0.5, 1.5])
+    for temperature in (1e-3, 0.7, 0.8, 1.25):
+        _check_grad(eng, z, tok, dtype, g, g * 0.5, g * 0.25, temperature, f"T {temperature}")
+
+
+@pytest.mark.parametrize("dtype,offset", [("f32", 2.0 ** 20), ("bf16", 128.0), ("f16", 1024.0)])
+@pytest.mark.parametrize("classes", [21, 300, 5000])
+def test_a_common_offset_changes_nothing(eng, dtype, offset, classes):
+    """z and z + offset, both exact in the type"""
+    from mica_amd import scoring
+    g = _rng(classes)
+    z = torch.randint(-4, 5, (6, classes), generator=g).float()
+    assert torch.equal((z + offset).to(DT[dtype]).float(), z + offset) and torch.equal((z - offset).to(DT[dtype]).float(), z - offset)
+    tok = torch.randint(0, classes, (6,), generator=g)
+    gl, ge = torch.randn((6,), generator=g), torch.randn((6,), generator=g)
+    zero = torch.zeros(6)
+    outs = []
+    for o in (0.0, offset, -offset):
+        x = (z + o).to(DT[dtype]).cuda().requires_grad_()
+        r = scoring.token_logprobs(eng, x, tok.cuda())
+        grad, = torch.autograd.grad([r.logprob, r.entropy], [x], [gl.cuda(), ge.cuda()])
+        outs.append((r.logprob.detach().cpu().double(), r.entropy.detach().cpu().double(), grad.cpu().double()))
+    want = so.score_grad(z, tok, gl, ge, None)
+    tol = _grad_tol(z, dtype, want, gl, ge, zero, 1.0)
+    for lp, ent, grad in outs[1:]:
+        _near(lp, outs[0][0], 2 * U * (_terms(classes) + 6 * outs[0][0].abs()))
+        _near(ent, outs[0][1], 2 * _herr(classes))
+        _near(grad, outs[0][2], 2 * tol)
+
+
+def test_c_entry_points_want_the_maxima_and_sums(eng):
+    """refused on the host, with a message; without a workspace rows are whole and a row's results do not depend on how many there are"""
+    import ctypes as C
+    from mica_amd import _cabi, scoring
+    z = torch.randn((300, 40000), generator=_rng(1)).cuda()
+    f = torch.empty((6, 300), device="cuda")
+
+    def call(v, rows, entropy, lse, aux):
+        return eng.lib.mica_token_logprobs_aux(eng._h, C.byref(v.desc), None, 0, -100, 1.0, 0, None, entropy.data_ptr(), lse.data_ptr(),
+                                               None if aux is None else aux.data_ptr(), None, None, None, 0, eng._raw_stream())
+    many, few = scoring.LogitsLayout(z, 1), scoring.LogitsLayout(z[:2], 1)
+    assert call(few, 2, f[0], f[1], None) == _cabi.MICA_ERR_ARG and b"mica_token_logprobs_aux" in eng.lib.mica_last_error(eng._h)
+    a, b = torch.zeros((2, 300), device="cuda"), torch.zeros((2, 2), device="cuda")
+    assert call(many, 300, f[0], f[1], a) == 0 and call(few, 2, f[2], f[3], b) == 0
+    assert torch.equal(a[:, :2], b) and torch.equal(f[0, :2], f[2, :2]) and torch.equal(a[0], z.amax(1))
+    assert eng.lib.mica_token_logprobs_backward(eng._h, C.byref(few.desc), None, 0, -100, 1.0, None, f[0].data_ptr(), None, f[0].data_ptr(), None,
+                                                z.data_ptr(), eng._raw_stream()) == _cabi.MICA_ERR_ARG
+    assert b"mica_token_logprobs_backward" in eng.lib.mica_last_error(eng._h)
