@@ -757,7 +757,8 @@ __device__ __forceinline__ RowGrad row_grad(const ScoreGrad& o, int64_t classes,
 }
 __device__ __forceinline__ float grad_value(const RowGrad& g, float z) {
     const float d = (z - g.m) * g.c;
-    return g.empty ? 0.f : exp2_hw(d) * fmaf(g.b, fmaxf(d, NEG_BIG), g.a);
+    // (2^d is 0 long before -1024; beyond it only the product with a large b, an entropy's scaled gradient at a small T, would overflow)
+    return g.empty ? 0.f : exp2_hw(d) * fmaf(g.b, fmaxf(d, -1024.f), g.a);
 }
 
 // what a block of the gradient kernels covers: G threads x UNROLL vectors of one row

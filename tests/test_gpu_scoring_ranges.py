@@ -294,3 +294,15 @@ def test_c_entry_points_want_the_maxima_and_sums(eng):
     assert eng.lib.mica_token_logprobs_backward(eng._h, C.byref(few.desc), None, 0, -100, 1.0, None, f[0].data_ptr(), None, f[0].data_ptr(), None,
                                                 z.data_ptr(), eng._raw_stream()) == _cabi.MICA_ERR_ARG
     assert b"mica_token_logprobs_backward" in eng.lib.mica_last_error(eng._h)
+
+
+@pytest.mark.parametrize("classes", [21, 300])
+def test_a_large_entropy_gradient_beside_masked_classes(eng, classes):
+    """an entropy gradient scaled by 2^16 at T = 1e-4: finite at classes of probability 0 (the product with their log p is 0)"""
+    z = torch.randn((3, classes), generator=_rng(classes)) * 1e-4
+    z[0, ::2] = NEG
+    z[1, ::2] = torch.finfo(torch.float32).min
+    z[2, 1:] = NEG
+    tok = torch.full((3,), -100)
+    zero, ge = torch.zeros(3), torch.tensor([65536.0, -65536.0, 65536.0])
+    _check_grad(eng, z, tok, "f32", zero, ge, zero, 1e-4)
