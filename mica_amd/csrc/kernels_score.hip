@@ -821,7 +821,7 @@ struct DistillArgs {
 struct RowGradient {
     float m, f;         // not listed: f 2^{z c - R(m)}, or f 2^{(z - m) c} beyond REF_MAX
     float M, qs;        // listed: qs 2^{(z - M) c} - sum p
-    float norm;         // log p = t - norm
+    float t0, norm;     // log p = (t - t0) - norm: the list's maximum and the log of its sum apart, as an offset of 1e8 would swallow the latter
     __device__ __forceinline__ bool empty() const { return M == -INFINITY; }
 };
 // The row's list in LDS: index (unused entries -1, no class: INT_MAX), log probability, logit.  Loaded by one wave.
@@ -893,10 +893,18 @@ __device__ __forceinline__ Online distill_stream(const T* __restrict__ z, int n,
     return on;
 }
 
+// the maximum of the list's values, 0 if that is -inf; one wave, in every lane
+__device__ __forceinline__ float list_max(const DistillArgs& a, ListLds d, int lane) {
+    float t = -INFINITY;
+    for (int k = lane; k < a.k; k += 64) t = fmaxf(t, d.t[k]);
+    t = wave_max(t);
+    return t == -INFINITY ? 0.f : t;
+}
 // What a row's list says by itself: one wave, in every lane.
 struct ListStats {
     double mass;        // sum p: of the renormalised list 1, or 0 if no entry has any; tail: sum of e^t
-    double norm;        // log sum of the values (renormalised), 0 (tail)
+    float t0;           // the values' maximum (renormalised; of no entry with any probability 0), 0 (tail)
+    double norm;        // log of the sum of e^{t - t0} (renormalised; -inf: none has any), 0 (tail)
     double log_sl;      // (tail) log of the listed classes' sum relative to zmax, every class once; -inf: none
     float zmax;
     int bad;            // an index that is no class
@@ -919,7 +927,8 @@ __device__ __forceinline__ ListStats list_stats(const DistillArgs& a, ListLds d,
         for (int k = lane; k < a.k; k += 64)
             if (d.i[k] >= 0) sum += tmax == -INFINITY ? (d.t[k] != d.t[k] ? (double)d.t[k] : 0.0) : exp((double)d.t[k] - tmax);
         sum = wave_sum(sum);
-        o.norm = sum == 0.0 ? -INFINITY : (tmax == -INFINITY ? sum : tmax + log(sum));
+        o.t0 = tmax == -INFINITY ? 0.f : tmax;
+        o.norm = tmax == -INFINITY && sum != 0.0 ? sum : log(sum);
         o.mass = sum == 0.0 ? 0.0 : 1.0;
     } else {
         double sl = 0.0, P = 0.0;
@@ -933,6 +942,7 @@ __device__ __forceinline__ ListStats list_stats(const DistillArgs& a, ListLds d,
         }
         o.log_sl = log(wave_sum(sl));
         o.mass = wave_sum(P);
+        o.t0 = 0.f;
         o.norm = 0.0;
     }
     return o;
@@ -968,6 +978,7 @@ __device__ __forceinline__ RowScalars row_scalars(const DistillArgs& a, const Li
     o.g.f = invalid ? NAN : (have_rest ? (float)(factor / s) : 0.f);
     o.g.M = (float)o.M;
     o.g.qs = invalid ? NAN : (o.M == -INFINITY ? 0.f : (float)(o.mass * exp(-o.log_s)));
+    o.g.t0 = l.t0;
     o.g.norm = (float)l.norm;
     if (invalid && o.M == -INFINITY) o.g.M = 0.f;               // a row of NaN is not an empty one
     return o;
@@ -977,7 +988,7 @@ __device__ __forceinline__ float row_loss(const DistillArgs& a, ListLds d, const
     double sum = 0.0;
     for (int k = lane; k < a.k; k += 64) {
         if (d.i[k] < 0) continue;
-        const double lp = (double)d.t[k] - l.norm;
+        const double lp = ((double)d.t[k] - l.t0) - l.norm;
         const double pk = o.mass == 0.0 ? 0.0 : exp(lp);
         const double lq = o.M == -INFINITY ? -INFINITY : ((double)d.z[k] - o.M) * a.inv_t - o.log_s;
         if (!(pk == 0.0)) sum += pk * (lp - lq);
@@ -1058,7 +1069,7 @@ __device__ __forceinline__ void listed_grad(const DistillArgs& a, T* __restrict_
         for (int j = 0; j < a.k; ++j) {
             if (d.i[j] != i) continue;
             again |= j < k;
-            p += a.tail ? expf(d.t[j]) : (q.norm == -INFINITY ? 0.f : expf(d.t[j] - q.norm));
+            p += a.tail ? expf(d.t[j]) : (q.norm == -INFINITY ? 0.f : expf((d.t[j] - q.t0) - q.norm));
         }
         if (!again) out[i] = from_f32<T>(scale * (q.qs * exp2_hw((d.z[k] - q.M) * a.c) - p));
     }
@@ -1083,6 +1094,7 @@ template <typename T, int G, int ONCE>
 __global__ __launch_bounds__(256) void distill_grad_row_kernel(LogitsView v, int64_t rows, DistillArgs a, int chunks, T* __restrict__ grad) {
     constexpr int GROUPS = 256 / G, CHUNK = G * UNROLL * Vec<T>::N;
     extern __shared__ int dyn[];
+    __shared__ float t0[GROUPS];
     const int g = threadIdx.x / G, tid = threadIdx.x % G;
     const int64_t item = (int64_t)blockIdx.x * GROUPS + g;
     if (item >= rows * chunks) return;
@@ -1091,15 +1103,20 @@ __global__ __launch_bounds__(256) void distill_grad_row_kernel(LogitsView v, int
     const ListLds list = list_lds(dyn + g * 3 * a.k, a.k);
     const RowPos p = row_pos(v, r);
     const T* z = static_cast<const T*>(v.p) + row_start(v, p);
-    if (tid < 64) list_load(a, list_pos(v, p, r, a.k), z, v.classes, tid, list);
+    if (tid < 64) {
+        list_load(a, list_pos(v, p, r, a.k), z, v.classes, tid, list);
+        const float t = a.tail ? 0.f : list_max(a, list, tid);      // of the entries that this lane has written
+        if (tid == 0) t0[g] = t;
+    }
     T* out = grad + r * v.classes;
     const float w = a.weight ? a.weight[r] : 1.f;
     const float scale = (a.g_loss ? a.g_loss[r] : 1.f) * w * a.t;
     const float x = a.aux[2 * rows + r], m = a.aux[r];
-    const RowGradient o{m, a.aux[rows + r], a.tail ? x : m, a.aux[3 * rows + r], a.tail ? 0.f : x};
+    RowGradient o{m, a.aux[rows + r], a.tail ? x : m, a.aux[3 * rows + r], 0.f, a.tail ? 0.f : x};
     const Unlisted unlisted(a, o, scale);
     map_chunk<T, G, ONCE>(z, out, first, v.classes, tid, [&](float y, int64_t) { return unlisted(y); });
     group_sync<G>();
+    o.t0 = t0[g];
     if (!unlisted.none) listed_grad<T, G>(a, out, list, first, CHUNK, o, scale, tid);
 }
 
@@ -1251,9 +1268,9 @@ __global__ __launch_bounds__(256) void distill_col_kernel(LogitsView v, int64_t 
     float z[CM], e[CM], target[CM];
     load_classes(z, static_cast<const T*>(v.p) + row_start(v, p), v.sc, classes);
     const float w = a.weight ? a.weight[r] : 1.f;
-    // the teacher: tail: p = e^t, r = 1 - sum p;  else p = e^{t - norm}
+    // the teacher: tail: p = e^t, r = 1 - sum p;  else p = e^{(t - t0) - norm}
     double total = 0.0;
-    float norm = 0.f;
+    float t0 = 0.f, norm = 0.f;
     if (a.tail) {
         for (int k = 0; k < a.k; ++k)
             if (load_int(a.index, l.base + k * l.stride, a.index_bytes) >= 0) total += exp((double)load_float(a.teacher, l.base + k * l.stride, a.teacher_dtype));
@@ -1266,7 +1283,8 @@ __global__ __launch_bounds__(256) void distill_col_kernel(LogitsView v, int64_t 
             const float t = load_float(a.teacher, l.base + k * l.stride, a.teacher_dtype);
             sum += tmax == -INFINITY ? (t != t ? t : 0.f) : exp2_hw((t - tmax) * LOG2E);
         }
-        norm = sum == 0.f ? -INFINITY : (tmax == -INFINITY ? sum : tmax + logf(sum));
+        t0 = tmax == -INFINITY ? 0.f : tmax;
+        norm = tmax == -INFINITY && sum != 0.f ? sum : logf(sum);
     }
     const bool nobody = !a.tail && norm == -INFINITY;                       // no entry has any probability
     const float m = max_of(z), ref = m == -INFINITY ? 0.f : m;
@@ -1286,7 +1304,7 @@ __global__ __launch_bounds__(256) void distill_col_kernel(LogitsView v, int64_t 
         const int64_t i = load_int(a.index, l.base + k * l.stride, a.index_bytes);
         if (i < 0) continue;
         if (i >= classes) { bad = true; continue; }
-        const float lp = load_float(a.teacher, l.base + k * l.stride, a.teacher_dtype) - norm;
+        const float lp = (load_float(a.teacher, l.base + k * l.stride, a.teacher_dtype) - t0) - norm;
         const float pk = nobody ? 0.f : exp2_hw(lp * LOG2E);
         listed |= 1ull << i;
         float zk = 0.f;

@@ -306,3 +306,22 @@ def test_a_large_entropy_gradient_beside_masked_classes(eng, classes):
     tok = torch.full((3,), -100)
     zero, ge = torch.zeros(3), torch.tensor([65536.0, -65536.0, 65536.0])
     _check_grad(eng, z, tok, "f32", zero, ge, zero, 1e-4)
+
+
+# ---- teachers' lists ---------------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("classes", [21, 65, 300, 5000, 70001])
+@pytest.mark.parametrize("offset", [0.0, 1e4, 1e6, 1e8, -1e8, -1e30])
+def test_a_constant_per_list_cancels(eng, classes, offset):
+    """values of any common magnitude: what is left of their distances after the addition counts, in the loss and in both gradients"""
+    g = _rng(classes)
+    z = torch.randn((5, classes), generator=g) * 3.0
+    idx = torch.stack([torch.randperm(classes, generator=g)[:5] for _ in range(5)]).int()
+    idx[1, 4] = -1
+    idx[2, 3] = idx[2, 0]
+    val = torch.tensor([0.0, -1.0, -2.0, -3.0, -0.5]).repeat(5, 1) + offset
+    val[3, 1] = NEG
+    val[4, 1:] = NEG
+    weight = torch.rand((5,), generator=g) + 0.5
+    for temperature in (1.0, 1.7):
+        _check_distill(eng, z, idx, val, "f32", temperature, False, weight, f"T {temperature}")
