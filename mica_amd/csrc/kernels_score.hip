@@ -949,7 +949,7 @@ __device__ __forceinline__ ListStats list_stats(const DistillArgs& a, ListLds d,
 }
 // The row's scalars from its list and the sums over all classes, or over those that are not listed (tail); any thread.  What cancels is
 // combined in float64: 1 - sum p, log q_rest = -log(1 + listed sum / rest sum).
-struct RowScalars { double M, log_s, rest, log_q_rest, mass; RowGradient g; };     // M, log_s: maximum and log sum of all classes
+struct RowScalars { double M, log_s, rest, log_q_rest, mass; bool invalid; RowGradient g; };     // M, log_s: maximum and log sum of all classes
 __device__ __forceinline__ RowScalars row_scalars(const DistillArgs& a, const ListStats& l, float m, float s) {
     RowScalars o;
     const double log_m = log_sum(m, s, a.c);                    // log of the streamed sum relative to m
@@ -973,18 +973,18 @@ __device__ __forceinline__ RowScalars row_scalars(const DistillArgs& a, const Li
         }
         factor = o.mass * exp(o.log_q_rest) - o.rest;
     }
-    const bool invalid = l.bad || s != s || o.log_s != o.log_s || o.mass != o.mass;      // shows in the gradient too
+    // a NaN anywhere, or an index that is no class: loss and gradient of the whole row are NaN
+    o.invalid = l.bad || s != s || o.log_s != o.log_s || o.mass != o.mass || l.norm != l.norm;
     o.g.m = a.tail && !have_rest ? 0.f : m;                    // without a tail M itself
-    o.g.f = invalid ? NAN : (have_rest ? (float)(factor / s) : 0.f);
+    o.g.f = have_rest ? (float)(factor / s) : 0.f;
     o.g.M = (float)o.M;
-    o.g.qs = invalid ? NAN : (o.M == -INFINITY ? 0.f : (float)(o.mass * exp(-o.log_s)));
+    o.g.qs = o.M == -INFINITY ? 0.f : (float)(o.mass * exp(-o.log_s));
     o.g.t0 = l.t0;
     o.g.norm = (float)l.norm;
-    if (invalid && o.M == -INFINITY) o.g.M = 0.f;               // a row of NaN is not an empty one
     return o;
 }
 // the loss; one wave, in every lane
-__device__ __forceinline__ float row_loss(const DistillArgs& a, ListLds d, const ListStats& l, const RowScalars& o, float s, int lane) {
+__device__ __forceinline__ float row_loss(const DistillArgs& a, ListLds d, const ListStats& l, const RowScalars& o, int lane) {
     double sum = 0.0;
     for (int k = lane; k < a.k; k += 64) {
         if (d.i[k] < 0) continue;
@@ -995,15 +995,18 @@ __device__ __forceinline__ float row_loss(const DistillArgs& a, ListLds d, const
     }
     sum = wave_sum(sum);
     if (o.rest > 0.0) sum += o.rest * (log(o.rest) - o.log_q_rest);
-    return l.bad || s != s ? NAN : (float)(sum * a.t * a.t);
+    return o.invalid ? NAN : (float)(sum * a.t * a.t);
 }
 // loss and aux of a row from its joined sums; one wave, the result in every lane
 __device__ __forceinline__ RowGradient finish_row(const DistillArgs& a, ListLds d, float m, float s, int64_t r, int64_t rows, int lane) {
     const ListStats l = list_stats(a, d, lane);
     const RowScalars o = row_scalars(a, l, m, s);
-    const float loss = row_loss(a, d, l, o, s, lane);
+    const float loss = row_loss(a, d, l, o, lane);
     RowGradient q = o.g;
-    if (loss != loss) q.f = q.qs = NAN;
+    if (loss != loss) {
+        q.f = q.qs = NAN;
+        if (q.empty()) q.m = q.M = 0.f;                         // or its gradient would be the empty row's, 0
+    }
     if (lane == 0) {
         const float w = a.weight ? a.weight[r] : 1.f;
         a.loss[r] = w == 0.f ? 0.f : loss * w;
@@ -1342,11 +1345,10 @@ __global__ __launch_bounds__(256) void distill_col_kernel(LogitsView v, int64_t 
         log_q_rest = shift + (LOSS ? log((double)s_rest) : (double)logf(s_rest)) - log_s;
         if (LOSS && rest > 0.f) sum += rest * (log((double)rest) - log_q_rest);
     }
-    const bool nan = bad || s != s || sum != sum;
+    const bool nan = bad || s != s || sum != sum || norm != norm || total != total;
     if (LOSS) a.loss[r] = w == 0.f ? 0.f : (nan ? NAN : (float)(sum * a.t * a.t)) * w;
     if (GRAD) {
         const float scale = (a.g_loss ? a.g_loss[r] : 1.f) * w * a.t;
-        const bool none = empty || w == 0.f;
         const float in_f = scale * mass / s, out_f = a.tail ? (s_rest > 0.f ? scale * (mass * expf((float)log_q_rest) - rest) / s_rest : 0.f) : in_f;
         T* out = grad + grad_start(v, p, r);
         const int64_t step = v.class_last ? 1 : v.inner;
@@ -1354,7 +1356,7 @@ __global__ __launch_bounds__(256) void distill_col_kernel(LogitsView v, int64_t 
         for (int c = 0; c < CM; ++c) {
             if (c < classes) {
                 const float d = (listed >> c) & 1 ? fmaf(in_f, e[c], -scale * target[c]) : out_f * e[c];
-                out[c * step] = from_f32<T>(none ? 0.f : (nan ? NAN : d));
+                out[c * step] = from_f32<T>(w == 0.f ? 0.f : (nan ? NAN : (empty ? 0.f : d)));
             }
         }
     }

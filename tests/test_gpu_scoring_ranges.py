@@ -325,3 +325,35 @@ def test_a_constant_per_list_cancels(eng, classes, offset):
     weight = torch.rand((5,), generator=g) + 0.5
     for temperature in (1.0, 1.7):
         _check_distill(eng, z, idx, val, "f32", temperature, False, weight, f"T {temperature}")
+
+
+@pytest.mark.parametrize("classes", [20, 64, 65, 300, 5000, 70001])
+@pytest.mark.parametrize("tail", [False, True])
+def test_what_makes_the_loss_nan_makes_the_whole_gradient_nan(eng, classes, tail):
+    """whatever the size and the entry point; and an empty row with a sound list keeps its loss of +inf and its gradient of 0"""
+    g = _rng(classes)
+    z = torch.randn((8, classes), generator=g)
+    idx = torch.stack([torch.randperm(classes, generator=g)[:4] for _ in range(8)]).int()
+    val = torch.log(torch.tensor([0.4, 0.3, 0.1, 0.05])).repeat(8, 1)
+    z[0] = NAN
+    z[1] = NEG
+    idx[1, 2] = classes                                       # no class
+    z[2] = NEG
+    val[2, 1] = NAN
+    val[3, 3] = NAN
+    z[4, int(idx[4, 0])] = NAN
+    val[4, 0] = NEG                                           # at a class that the list gives no probability
+    idx[5, 0] = classes + 5
+    z[6] = NEG
+    nan = [0, 1, 2, 3, 4, 5]
+    d = [t.cuda() for t in (z, idx, val)]
+    ones = torch.ones(8, device="cuda")
+    loss, aux = eng.distill_loss(*d, tail=tail)
+    back = eng.distill_backward(*d, aux, ones, tail=tail)
+    sl, sg = eng.distill_step(*d, tail=tail)
+    for lo, gr in ((loss, back), (sl, sg)):
+        assert torch.isnan(lo).nonzero()[:, 0].tolist() == nan
+        assert bool(torch.isnan(gr[nan]).all()) and not bool(torch.isnan(gr[6:]).any())
+        assert math.isinf(float(lo[6])) and float(lo[6]) > 0 and float(gr[6].abs().max()) == 0.0
+    want, wgrad, _ = so.distill(z[7:], idx[7:], val[7:], 1.0, tail)
+    assert float((loss[7:].cpu() - want).abs()) < U * 2 * _terms(classes) and float((back[7:].cpu() - wgrad).abs().max()) < U * 2 * _terms(classes)
