@@ -298,7 +298,7 @@ typedef struct mica_top_list {
 int64_t mica_distill_ws(const mica_logits* z, int step);            /* bytes for mica_distill_loss (step = 0) / mica_distill_step (1) */
 int mica_distill_loss(mica_ctx* ctx, const mica_logits* z, const mica_top_list* list, float temperature, float* d_loss, float* d_aux,
                       void* d_ws, int64_t ws_bytes, void* stream);
-/* d_grad = gradient of sum_n g_loss loss with respect to the logits */
+/* d_grad = gradient of sum_n g_loss loss with respect to the logits; 0 in a row whose g_loss is 0, whatever the row holds */
 int mica_distill_backward(mica_ctx* ctx, const mica_logits* z, const mica_top_list* list, float temperature, const float* d_aux,
                           const float* d_g_loss, void* d_grad, void* stream);
 /* Loss and gradient of a training step in one call: d_loss = weight loss, d_grad = gradient of sum_n weight_n loss_n; d_weight f32[rows]

@@ -1356,7 +1356,7 @@ __global__ __launch_bounds__(256) void distill_col_kernel(LogitsView v, int64_t 
         for (int c = 0; c < CM; ++c) {
             if (c < classes) {
                 const float d = (listed >> c) & 1 ? fmaf(in_f, e[c], -scale * target[c]) : out_f * e[c];
-                out[c * step] = from_f32<T>(w == 0.f ? 0.f : (nan ? NAN : (empty ? 0.f : d)));
+                out[c * step] = from_f32<T>(scale == 0.f ? 0.f : (nan ? NAN : (empty ? 0.f : d)));
             }
         }
     }

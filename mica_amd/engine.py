@@ -501,7 +501,8 @@ class Engine:
 
     def distill_backward(self, student, teacher_index, teacher_logprob, aux, g_loss, dim: int = -1, temperature: float = 1.0, tail: bool = False,
                          view=None):
-        """Gradient, in the student's type and shape, of (g_loss * loss).sum(); aux: distill_loss' second result for the same arguments."""
+        """Gradient, in the student's type and shape, of (g_loss * loss).sum(); aux: distill_loss' second result for the same arguments.
+        A row whose g_loss is 0 has gradient 0 whatever it holds."""
         v = self.logits_view(student, dim, "student") if view is None else view
         temperature = scoring.check_temperature(temperature)
         lst, keep = scoring.top_list(v, teacher_index, teacher_logprob, tail, self.device)

@@ -357,3 +357,23 @@ def test_what_makes_the_loss_nan_makes_the_whole_gradient_nan(eng, classes, tail
         assert math.isinf(float(lo[6])) and float(lo[6]) > 0 and float(gr[6].abs().max()) == 0.0
     want, wgrad, _ = so.distill(z[7:], idx[7:], val[7:], 1.0, tail)
     assert float((loss[7:].cpu() - want).abs()) < U * 2 * _terms(classes) and float((back[7:].cpu() - wgrad).abs().max()) < U * 2 * _terms(classes)
+
+
+@pytest.mark.parametrize("classes", [20, 64, 65, 300, 5000])
+@pytest.mark.parametrize("tail", [False, True])
+def test_a_masked_loss_has_gradient_zero_whatever_the_row_holds(eng, classes, tail):
+    """through the loss's upstream gradient and through the step's weight, at both sides of 64 classes"""
+    from mica_amd import scoring
+    z = torch.randn((4, classes), generator=_rng(classes))
+    idx = torch.arange(3).repeat(4, 1).int()
+    val = torch.log(torch.tensor([0.4, 0.3, 0.1])).repeat(4, 1)
+    z[0] = NAN
+    idx[1, 0] = classes
+    val[2, 0] = NAN
+    mask = torch.tensor([0.0, 0.0, 0.0, 1.0]).cuda()
+    x = z.cuda().requires_grad_()
+    loss = scoring.distill_loss(eng, x, idx.cuda(), val.cuda(), tail=tail)
+    torch.where(mask > 0, loss, torch.zeros_like(loss)).sum().backward()
+    _, sg = eng.distill_step(z.cuda(), idx.cuda(), val.cuda(), tail=tail, weight=mask)
+    for grad in (x.grad, sg):
+        assert float(grad[:3].abs().max()) == 0.0 and bool(torch.isfinite(grad[3]).all()) and float(grad[3].abs().max()) > 0.0
