@@ -54,7 +54,7 @@ class LogitsLayout:
     """How a logits tensor is handed to the library: the view (`desc`), the tensor it points into (`base`: the logits themselves, or a
     copy where no view fits), and the shapes of what comes back.  `moved`: the copy has the class axis last, results are laid out like
     it and returned as views with the axis where the caller has it."""
-    __slots__ = ("dim", "shape", "classes", "rows_shape", "rows", "base", "moved", "class_last", "desc", "dtype")
+    __slots__ = ("dim", "shape", "classes", "rows_shape", "rows", "base", "moved", "class_last", "desc", "dtype", "strides", "device")
 
     def __init__(self, logits: torch.Tensor, dim: int):
         dtype = DTYPES.get(logits.dtype) if isinstance(logits, torch.Tensor) else None
@@ -64,7 +64,7 @@ class LogitsLayout:
         if not shape or not -len(shape) <= dim < len(shape):
             raise MicaHipError(f"dim {dim} is no axis of logits of shape {shape}")
         self.dim = dim = dim % len(shape)
-        self.shape, self.dtype = shape, logits.dtype
+        self.shape, self.dtype, self.device = shape, logits.dtype, logits.device
         self.classes = classes = shape[dim]
         self.rows_shape = rows_shape = shape[:dim] + shape[dim + 1:]
         self.rows = rows = math.prod(rows_shape)
@@ -85,7 +85,21 @@ class LogitsLayout:
                     self.base = logits.contiguous()
                     view = self._view(self.base, dim)
             outer, inner, self.class_last, sc = view
+        self.strides = self.base.stride()
         self.desc = _cabi.MicaLogits(self.base.data_ptr(), dtype, self.class_last, outer[0], inner[0], classes, outer[1], inner[1], sc)
+
+    def release(self):
+        """-> the tensor the view points into, for autograd to keep: the layout stays behind with sizes and strides alone"""
+        base, self.base = self.base, None
+        return base
+
+    def over(self, base):
+        """this layout of `base`, a tensor of release()'s values: that tensor itself, or what a saved-tensor hook made of it"""
+        if base.data_ptr() == self.desc.d_data and base.stride() == self.strides:
+            return self
+        v = LogitsLayout(base, base.dim() - 1 if self.moved else self.dim)
+        v.dim, v.shape, v.rows_shape, v.moved = self.dim, self.shape, self.rows_shape, self.moved
+        return v
 
     @staticmethod
     def _view(t, dim):
@@ -104,7 +118,7 @@ class LogitsLayout:
 
     def score_aux(self):
         """what token_logprobs hands to its backward pass: maximum and sum of every row; None for few classes, which a thread sums again"""
-        return torch.empty((2, self.rows), dtype=torch.float32, device=self.base.device) if self.classes > COL_MAX else None
+        return torch.empty((2, self.rows), dtype=torch.float32, device=self.device) if self.classes > COL_MAX else None
 
     def with_axis(self, k):
         """shape with k entries at the class axis, as the library lays it out"""
@@ -160,9 +174,10 @@ class _TokenLogprobs(torch.autograd.Function):
         view = engine.logits_view(logits, dim)
         aux = view.score_aux()
         r = engine.token_logprobs(logits, tokens, top, dim, temperature, ignore_index, view, aux)
+        # every tensor through save_for_backward: torch frees them after the backward pass, refuses one over logits that were written since,
+        # and lets hooks keep them elsewhere
+        ctx.save_for_backward(view.release(), r.lse, r.entropy, tokens, aux)
         ctx.call = engine, view, temperature, ignore_index, dim
-        # through save_for_backward, also what the view points into: torch refuses a backward pass over logits that were written since
-        ctx.save_for_backward(logits, r.lse, r.entropy, tokens, aux)
         if r.top_index is not None:
             ctx.mark_non_differentiable(r.top_logprob, r.top_index)
         ctx.set_materialize_grads(False)
@@ -173,9 +188,10 @@ class _TokenLogprobs(torch.autograd.Function):
     def backward(ctx, g_logprob, g_entropy, g_lse, *_):
         if g_logprob is None and g_entropy is None and g_lse is None:
             return (None,) * 7
-        logits, lse, entropy, tokens, aux = ctx.saved_tensors
+        base, lse, entropy, tokens, aux = ctx.saved_tensors
         engine, view, temperature, ignore_index, dim = ctx.call
-        return (engine.token_logprobs_backward(logits, tokens, lse, entropy, g_logprob, g_entropy, g_lse, dim, temperature, ignore_index, view, aux),
+        view = view.over(base)
+        return (engine.token_logprobs_backward(base, tokens, lse, entropy, g_logprob, g_entropy, g_lse, dim, temperature, ignore_index, view, aux),
                 None, None, None, None, None, None)
 
 
@@ -189,16 +205,16 @@ class _DistillLoss(torch.autograd.Function):
     def forward(ctx, student, engine, index, logprob, dim, temperature, tail):
         view = engine.logits_view(student, dim, "student")
         loss, aux = engine.distill_loss(student, index, logprob, dim, temperature, tail, view)
+        ctx.save_for_backward(view.release(), index, logprob, aux)
         ctx.call = engine, view, dim, temperature, tail
-        ctx.save_for_backward(student, index, logprob, aux)
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_loss):
-        student, index, logprob, aux = ctx.saved_tensors
+        base, index, logprob, aux = ctx.saved_tensors
         engine, view, dim, temperature, tail = ctx.call
-        return (engine.distill_backward(student, index, logprob, aux, g_loss, dim, temperature, tail, view), None, None, None, None, None, None)
+        return (engine.distill_backward(base, index, logprob, aux, g_loss, dim, temperature, tail, view.over(base)), None, None, None, None, None, None)
 
 
 def distill_loss(engine, student, teacher_index, teacher_logprob, dim: int = -1, temperature: float = 1.0, tail: bool = False) -> torch.Tensor:

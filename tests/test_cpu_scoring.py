@@ -1,7 +1,9 @@
 """Class scoring and distillation without a GPU: the oracle's gradients against differences, the view of a logits tensor that is handed
 to the library, the library's own argument checks, and what the engine refuses."""
 import ctypes as C
+import gc
 import threading
+import weakref
 
 import pytest
 import torch
@@ -240,3 +242,87 @@ def test_the_gradients_maxima_and_sums_are_checked(eng):
         eng.token_logprobs(z[:, :64], tok, aux=torch.zeros(2, 4))
     lib = _lib()
     assert lib.mica_token_logprobs_aux(None, C.byref(_desc()), None, 0, -100, 1.0, 0, None, None, None, None, None, None, None, 0, None) == _cabi.MICA_ERR_ARG
+
+
+class _TorchEngine:
+    """the engine's calls of the autograd functions, on the CPU: gradients read through the view that is handed to the library"""
+    device = torch.device("cpu")
+
+    def __init__(self):
+        self.bases = []
+
+    def logits_view(self, logits, dim, name="logits"):
+        v = scoring.LogitsLayout(logits, dim)
+        self.bases.append(weakref.ref(v.base))
+        return v
+
+    def _rows(self, view, saved=None):
+        """the logits as the description alone says: [outer, inner, classes]"""
+        d, base = view.desc, saved if view.base is None else view.base
+        assert d.d_data == base.data_ptr()
+        return base.as_strided((d.outer, d.inner, d.classes), (d.stride_outer, d.stride_inner, d.stride_class), base.storage_offset()).double()
+
+    def _give(self, g, view):
+        return view.give((g if view.class_last else g.transpose(1, 2)).reshape(view.with_axis(view.classes)).to(view.dtype))
+
+    def token_logprobs(self, logits, tokens, top, dim, temperature, ignore_index, view, aux):
+        lse = torch.logsumexp(self._rows(view), -1).reshape(view.rows_shape).float()
+        return scoring.TokenScores(None if tokens is None else lse * 0, lse * 0, lse, None, None)
+
+    def token_logprobs_backward(self, logits, tokens, lse, entropy, g_logprob, g_entropy, g_lse, dim, temperature, ignore_index, view, aux):
+        z = self._rows(view, logits)
+        return self._give(torch.softmax(z, -1) * g_lse.reshape(z.shape[:2])[..., None], view)
+
+    def distill_loss(self, student, index, logprob, dim, temperature, tail, view):
+        lse = torch.logsumexp(self._rows(view), -1).reshape(view.rows_shape).float()
+        return lse, torch.zeros(4, view.rows)
+
+    def distill_backward(self, student, index, logprob, aux, g_loss, dim, temperature, tail, view):
+        z = self._rows(view, student)
+        return self._give(torch.softmax(z, -1) * g_loss.reshape(z.shape[:2])[..., None], view)
+
+
+AUTOGRAD_LAYOUTS = [(lambda x: x, (6, 100), 1), (lambda x: x[:, 1:], (2, 21, 3, 4), 1), (lambda x: x, (3, 100, 5), 1), (lambda x: x[:, :-1], (3, 6, 90), 2),
+                    (lambda x: x[..., ::2], (4, 200), 1)]
+
+
+def _scoring_calls(engine, dim):
+    idx, val = torch.zeros(1, dtype=torch.int64), torch.zeros(1)
+    return (lambda y: scoring.token_logprobs(engine, y, None, dim=dim).lse, lambda y: scoring.distill_loss(engine, y, idx, val, dim=dim))
+
+
+@pytest.mark.parametrize("cut,shape,dim", AUTOGRAD_LAYOUTS)
+def test_logits_are_freed_with_the_backward_pass(cut, shape, dim):
+    """a loss that the caller keeps keeps neither the logits nor a copy of them"""
+    for which in (0, 1):
+        engine = _TorchEngine()
+        x = torch.randn(shape, generator=torch.Generator().manual_seed(1)).requires_grad_()
+        y = cut(x * 1.0)
+        ref = weakref.ref(y)
+        loss = _scoring_calls(engine, dim)[which](y).sum()
+        del y
+        loss.backward()
+        gc.collect()
+        assert loss.grad_fn is not None and ref() is None and engine.bases[0]() is None
+        want, = torch.autograd.grad(torch.logsumexp(cut(x * 1.0), dim).sum(), x)
+        assert float((x.grad - want).abs().max()) < 1e-6
+
+
+@pytest.mark.parametrize("cut,shape,dim", AUTOGRAD_LAYOUTS)
+def test_the_backward_pass_reads_what_saved_tensor_hooks_give_back(cut, shape, dim):
+    """packed elsewhere and given back at another address, with other strides"""
+    for which in (0, 1):
+        x = torch.randn(shape, generator=torch.Generator().manual_seed(2)).requires_grad_()
+        given = []
+
+        def unpack(t):
+            given.append(t.clone(memory_format=torch.contiguous_format))
+            return given[-1]
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach().clone(memory_format=torch.contiguous_format), unpack):
+            y = cut(x * 1.0)
+            loss = _scoring_calls(_TorchEngine(), dim)[which](y).sum()
+        with torch.no_grad():
+            y.zero_()                                       # what was packed is what counts
+        loss.backward()
+        want, = torch.autograd.grad(torch.logsumexp(cut(x * 1.0), dim).sum(), x)
+        assert given and float((x.grad - want).abs().max()) < 1e-6

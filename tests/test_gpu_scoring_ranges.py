@@ -377,3 +377,35 @@ def test_a_masked_loss_has_gradient_zero_whatever_the_row_holds(eng, classes, ta
     _, sg = eng.distill_step(z.cuda(), idx.cuda(), val.cuda(), tail=tail, weight=mask)
     for grad in (x.grad, sg):
         assert float(grad[:3].abs().max()) == 0.0 and bool(torch.isfinite(grad[3]).all()) and float(grad[3].abs().max()) > 0.0
+
+
+# ---- what autograd keeps ------------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("shape,dim,cut", [((3, 9, 501), 2, lambda x: x[:, :-1]), ((2, 21, 4, 4, 4), 1, lambda x: x[:, 1:]), ((3, 400, 5), 1, lambda x: x)])
+def test_saved_logits_may_be_kept_on_the_host_and_are_freed(eng, shape, dim, cut):
+    from mica_amd import scoring
+    x = torch.randn(shape, generator=_rng(3)).cuda()
+    z = cut(x)
+    tok = torch.zeros(z.shape[:dim] + z.shape[dim + 1:], dtype=torch.int64, device="cuda")
+    lists = z.shape[:dim] + (2,) + z.shape[dim + 1:]
+    idx = torch.arange(2, device="cuda").view([2 if a == dim else 1 for a in range(len(lists))]).expand(lists).int()
+    val = torch.full(lists, math.log(0.4), device="cuda")
+
+    def grads(ctx):
+        leaf = x.clone().requires_grad_()
+        with ctx():
+            a = scoring.token_logprobs(eng, cut(leaf * 1.0), tok, dim=dim)
+            loss = (a.logprob + a.entropy).sum() + scoring.distill_loss(eng, cut(leaf * 1.0), idx, val, dim=dim, tail=True).sum()
+        loss.backward()
+        return loss, leaf.grad
+    import contextlib
+    _, want = grads(contextlib.nullcontext)
+    _, got = grads(lambda: torch.autograd.graph.save_on_cpu(pin_memory=False))
+    assert torch.equal(got, want)
+    # a loss that is kept after its backward pass keeps no logits
+    big = torch.randn((512, 16384), device="cuda").requires_grad_()
+    before = torch.cuda.memory_allocated()
+    kept = scoring.token_logprobs(eng, big * 1.0, torch.zeros(512, dtype=torch.int64, device="cuda")).logprob.sum()
+    kept.backward()
+    big.grad = None
+    assert kept.grad_fn is not None and torch.cuda.memory_allocated() - before < 1 << 20
