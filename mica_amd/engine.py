@@ -404,13 +404,17 @@ class Engine:
         probabilities and lse -inf, entropy 0 (any other row's lse is kept within float32).  Asynchronous; the results have no autograd
         history (scoring.token_logprobs has).  aux: of logits_view(logits, dim).score_aux(), written for token_logprobs_backward."""
         v = self.logits_view(logits, dim) if view is None else view
+        if aux is not None:
+            self._check_score_aux(aux, v)
+        return self._scores(v, tokens, top, temperature, ignore_index, aux)
+
+    def _scores(self, v, tokens, top, temperature, ignore_index, aux):
+        """token_logprobs of a view, with v.score_aux() or None; the caller holds call_lock"""
         temperature = scoring.check_temperature(temperature)
         top = int(top)
         if not 0 <= top <= min(scoring.MAX_TOP, v.classes):
             raise MicaHipError(f"top must be in [0, {min(scoring.MAX_TOP, v.classes)}], got {top}")
         dev, shape = self.device, v.rows_shape
-        if aux is not None:
-            self._check_score_aux(aux, v)
         logprob = topv = topi = None
         if tokens is not None:
             tokens = scoring.check_ints(tokens, "tokens", shape, dev).contiguous()
@@ -449,19 +453,27 @@ class Engine:
         v = self.logits_view(logits, dim) if view is None else view
         temperature = scoring.check_temperature(temperature)
         dev, shape = self.device, v.rows_shape
-        lse = scoring.check_floats(lse, "lse", shape, dev).contiguous()
-        entropy = scoring.check_floats(entropy, "entropy", shape, dev).contiguous()
-        if g_entropy is not None:
-            g_entropy = scoring.check_floats(g_entropy, "g_entropy", shape, dev).contiguous()
-        if g_lse is not None:
-            g_lse = scoring.check_floats(g_lse, "g_lse", shape, dev).contiguous()
+        scoring.check_floats(lse, "lse", shape, dev)
+        scoring.check_floats(entropy, "entropy", shape, dev)
+        for g, name in ((g_logprob, "g_logprob"), (g_entropy, "g_entropy"), (g_lse, "g_lse")):
+            if g is not None:
+                scoring.check_floats(g, name, shape, dev)
         if g_logprob is not None:
-            g_logprob = scoring.check_floats(g_logprob, "g_logprob", shape, dev).contiguous()
-            tokens = scoring.check_ints(tokens, "tokens", shape, dev).contiguous()
-        else:
-            tokens = None
+            scoring.check_ints(tokens, "tokens", shape, dev)
         if aux is not None:
             self._check_score_aux(aux, v)
+        return self._score_gradient(v, tokens, aux, entropy, g_logprob, g_entropy, g_lse, temperature, ignore_index)
+
+    def _score_gradient(self, v, tokens, aux, entropy, g_logprob, g_entropy, g_lse, temperature, ignore_index):
+        """token_logprobs_backward of tensors that are known to fit the view; the caller holds call_lock"""
+        dev = self.device
+        entropy = entropy.contiguous()
+        g_entropy = None if g_entropy is None else g_entropy.contiguous()
+        g_lse = None if g_lse is None else g_lse.contiguous()
+        if g_logprob is not None:
+            g_logprob, tokens = g_logprob.contiguous(), tokens.contiguous()
+        else:
+            tokens = None
         grad = torch.empty(v.with_axis(v.classes), dtype=v.dtype, device=dev)
         if v.rows:
             z = C.byref(v.desc)

@@ -173,11 +173,12 @@ class _TokenLogprobs(torch.autograd.Function):
     def forward(ctx, logits, engine, tokens, top, dim, temperature, ignore_index):
         view = engine.logits_view(logits, dim)
         aux = view.score_aux()
-        r = engine.token_logprobs(logits, tokens, top, dim, temperature, ignore_index, view, aux)
+        with engine.call_lock:
+            r = engine._scores(view, tokens, top, temperature, ignore_index, aux)
         # every tensor through save_for_backward: torch frees them after the backward pass, refuses one over logits that were written since,
         # and lets hooks keep them elsewhere
-        ctx.save_for_backward(view.release(), r.lse, r.entropy, tokens, aux)
-        ctx.call = engine, view, temperature, ignore_index, dim
+        ctx.save_for_backward(view.release(), r.entropy, tokens, aux)
+        ctx.call = engine, view, float(temperature), ignore_index
         if r.top_index is not None:
             ctx.mark_non_differentiable(r.top_logprob, r.top_index)
         ctx.set_materialize_grads(False)
@@ -188,11 +189,11 @@ class _TokenLogprobs(torch.autograd.Function):
     def backward(ctx, g_logprob, g_entropy, g_lse, *_):
         if g_logprob is None and g_entropy is None and g_lse is None:
             return (None,) * 7
-        base, lse, entropy, tokens, aux = ctx.saved_tensors
-        engine, view, temperature, ignore_index, dim = ctx.call
-        view = view.over(base)
-        return (engine.token_logprobs_backward(base, tokens, lse, entropy, g_logprob, g_entropy, g_lse, dim, temperature, ignore_index, view, aux),
-                None, None, None, None, None, None)
+        base, entropy, tokens, aux = ctx.saved_tensors
+        engine, view, temperature, ignore_index = ctx.call
+        with engine.call_lock:
+            grad = engine._score_gradient(view.over(base), tokens, aux, entropy, g_logprob, g_entropy, g_lse, temperature, ignore_index)
+        return grad, None, None, None, None, None, None
 
 
 def token_logprobs(engine, logits, tokens=None, top: int = 0, dim: int = -1, temperature: float = 1.0, ignore_index: int = -100) -> TokenScores:

@@ -249,28 +249,29 @@ class _TorchEngine:
     device = torch.device("cpu")
 
     def __init__(self):
-        self.bases = []
+        self.bases, self.call_lock = [], threading.RLock()
 
     def logits_view(self, logits, dim, name="logits"):
         v = scoring.LogitsLayout(logits, dim)
         self.bases.append(weakref.ref(v.base))
         return v
 
-    def _rows(self, view, saved=None):
-        """the logits as the description alone says: [outer, inner, classes]"""
-        d, base = view.desc, saved if view.base is None else view.base
-        assert d.d_data == base.data_ptr()
-        return base.as_strided((d.outer, d.inner, d.classes), (d.stride_outer, d.stride_inner, d.stride_class), base.storage_offset()).double()
+    def _rows(self, view):
+        """the logits at the description's address alone: [outer, inner, classes]"""
+        d = view.desc
+        n = 1 + (d.outer - 1) * d.stride_outer + (d.inner - 1) * d.stride_inner + (d.classes - 1) * d.stride_class
+        flat = torch.frombuffer((C.c_float * n).from_address(d.d_data), dtype=torch.float32)
+        return flat.as_strided((d.outer, d.inner, d.classes), (d.stride_outer, d.stride_inner, d.stride_class)).double()
 
     def _give(self, g, view):
         return view.give((g if view.class_last else g.transpose(1, 2)).reshape(view.with_axis(view.classes)).to(view.dtype))
 
-    def token_logprobs(self, logits, tokens, top, dim, temperature, ignore_index, view, aux):
+    def _scores(self, view, tokens, top, temperature, ignore_index, aux):
         lse = torch.logsumexp(self._rows(view), -1).reshape(view.rows_shape).float()
         return scoring.TokenScores(None if tokens is None else lse * 0, lse * 0, lse, None, None)
 
-    def token_logprobs_backward(self, logits, tokens, lse, entropy, g_logprob, g_entropy, g_lse, dim, temperature, ignore_index, view, aux):
-        z = self._rows(view, logits)
+    def _score_gradient(self, view, tokens, aux, entropy, g_logprob, g_entropy, g_lse, temperature, ignore_index):
+        z = self._rows(view)
         return self._give(torch.softmax(z, -1) * g_lse.reshape(z.shape[:2])[..., None], view)
 
     def distill_loss(self, student, index, logprob, dim, temperature, tail, view):
@@ -278,7 +279,7 @@ class _TorchEngine:
         return lse, torch.zeros(4, view.rows)
 
     def distill_backward(self, student, index, logprob, aux, g_loss, dim, temperature, tail, view):
-        z = self._rows(view, student)
+        z = self._rows(view)
         return self._give(torch.softmax(z, -1) * g_loss.reshape(z.shape[:2])[..., None], view)
 
 
