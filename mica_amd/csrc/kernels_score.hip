@@ -202,9 +202,7 @@ __device__ __forceinline__ float ref_residue(float m, float c) {
 // exponent between the references of two maxima, old <= now; -inf - -inf and the like end at NEG_BIG (with empty sums)
 __device__ __forceinline__ float ref_step(float old, float now, float c) {
 #pragma clang fp contract(off)
-    const float a = reference(old, c), b = reference(now, c);
-    const float d = ref_near(a) && ref_near(b) ? a - b : (old - now) * c + (ref_residue(now, c) - ref_residue(old, c));
-    return fmaxf(d, NEG_BIG);
+    return fmaxf((old - now) * c + (ref_residue(now, c) - ref_residue(old, c)), NEG_BIG);
 }
 // log of sum_v e^{(z_v - m) / T}; -inf for an empty row
 __device__ __forceinline__ double log_sum(float m, double s, float c) { return log(s) - (double)ref_residue(m, c) * LN2; }
@@ -231,14 +229,13 @@ struct Online {
     // N logits, vmax their maximum (never NaN).  All lanes of a wave call it together.
     template <int N, bool ENT> __device__ __forceinline__ void add(const float (&f)[N], float vmax, float c) {
         const float mn = fmaxf(m, vmax), R = reference(mn, c), old = reference(m, c);
-        // some lane's maximum is -inf or of large magnitude, or was so and its sums still count
-        if (__builtin_expect(__any(!ref_near(R) || !ref_near(fmaxf(old, R - REF_STEP))), 0)) {
+        // some lane's maximum is -inf or of large magnitude, or may have been so while its sums still count
+        if (__builtin_expect(__any(!(fabsf(R) <= REF_MAX - REF_STEP)), 0)) {
             rescale(mn, c);
-            const bool none = mn == -INFINITY, far = !ref_near(R) && !none;
-            const float ref = far || none ? 0.f : R, sub = far ? mn : 0.f;
+            const float ref = ref_near(R) ? R : 0.f, sub = ref_near(R) || mn == -INFINITY ? 0.f : mn;
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                const float x = far ? (f[j] - sub) * c : fmaf(f[j], c, -ref);
+                const float x = fmaf(f[j] - sub, c, -ref);
                 const float e = exp2_hw(x);
                 s += e;
                 if (ENT) w = fmaf(e, fmaxf(x, NEG_BIG), w);
@@ -603,9 +600,10 @@ __device__ __forceinline__ void write_top(const ScoreOut& o, const LogitsView& v
 
 // One read of the logits.  HBM-bound without alternatives: 4096 x 128000 bf16 175 us = 6.0 TB/s (a bare read of it 152-175 us), 7.6
 // instructions and one exponential per logit, half of the issue slots.  With alternatives the selection behind the stream is not hidden
-// by the other blocks of the CU: 227 us for K = 20.  Two vectors at a time then, which leaves registers for six blocks.
+// by the other blocks of the CU: 227 us for K = 20.  Two vectors at a time then, which leaves registers for six blocks.  (The waves per SIMD
+// in the bounds here and of the other kernels are what the stream's own registers allow; the path of far rows would cost one wave.)
 template <typename T, int G, bool TOP, int ONCE>
-__global__ __launch_bounds__(256) void score_row_kernel(LogitsView v, int64_t rows, ScoreOut o, int segments, int seg_len, Partial* __restrict__ part,
+__global__ __launch_bounds__(256, sizeof(T) == 4 && !TOP ? 8 : 6) void score_row_kernel(LogitsView v, int64_t rows, ScoreOut o, int segments, int seg_len, Partial* __restrict__ part,
                                                         u64* __restrict__ part_top) {
     constexpr int N = Vec<T>::N, NW = G / 64, GROUPS = 256 / G, U = TOP ? 2 : UNROLL;
     __shared__ Partial waves[4];
@@ -964,12 +962,12 @@ __device__ __forceinline__ RowScalars row_scalars(const DistillArgs& a, const Li
         o.mass += o.rest;
         if (!have_rest) { o.M = l.zmax; o.log_s = l.log_sl; }
         else if (l.log_sl != -INFINITY) {
+            // the two parts of the row's sum, relative to M: the larger one is about 1 or more, which the smaller one's log does not swallow
             o.M = fmaxf(m, l.zmax);
-            const double u = ((double)l.zmax - m) * a.inv_t + l.log_sl - log_m;      // log of (listed sum / rest sum)
-            o.log_q_rest = -(u > 700.0 ? u : log1p(exp(u)));
-            // relative to M, as two parts of which the larger one is about 1 or more: through u, a listed class 1e12 above would swallow it
-            const double r = ((double)m - o.M) * a.inv_t + log_m, t = ((double)l.zmax - o.M) * a.inv_t + l.log_sl;
-            o.log_s = fmax(r, t) + log1p(exp(-fabs(r - t)));
+            const double r = ((double)m - o.M) * a.inv_t + log_m, t = ((double)l.zmax - o.M) * a.inv_t + l.log_sl, u = t - r;
+            const double v = log1p(exp(-fabs(u)));
+            o.log_q_rest = -(fmax(u, 0.0) + v);
+            o.log_s = fmax(r, t) + v;
         }
         factor = o.mass * exp(o.log_q_rest) - o.rest;
     }
@@ -1023,7 +1021,7 @@ __device__ __forceinline__ RowGradient finish_row(const DistillArgs& a, ListLds 
 // One read of the logits, a bit of LDS per class to leave out the listed ones (tail; subtracting them afterwards would cancel for every
 // good student).  HBM-bound: 4096 x 128000 bf16 174 us = 6.0 TB/s, 180 with the tail; 513 x 32003 15 us, the latency of its steps.
 template <typename T, int G, bool TAIL, int ONCE>
-__global__ __launch_bounds__(256) void distill_row_kernel(LogitsView v, int64_t rows, DistillArgs a, int segments, int seg_len, Partial* __restrict__ part) {
+__global__ __launch_bounds__(256, (sizeof(T) == 4 ? 7 : 5) + (G == 256)) void distill_row_kernel(LogitsView v, int64_t rows, DistillArgs a, int segments, int seg_len, Partial* __restrict__ part) {
     constexpr int GROUPS = 256 / G;
     extern __shared__ int dyn[];
     __shared__ Partial waves[4];
@@ -1239,7 +1237,7 @@ __global__ __launch_bounds__(256) void score_col_kernel(LogitsView v, int64_t ro
 __device__ __forceinline__ int64_t grad_start(const LogitsView& v, RowPos p, int64_t r) { return v.class_last ? r * v.classes : p.outer * v.classes * v.inner + p.inner; }
 
 template <typename T, int CM>
-__global__ __launch_bounds__(256) void score_grad_col_kernel(LogitsView v, int64_t rows, ScoreGrad o, T* __restrict__ grad) {
+__global__ __launch_bounds__(256, 6) void score_grad_col_kernel(LogitsView v, int64_t rows, ScoreGrad o, T* __restrict__ grad) {
     const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (r >= rows) return;
     const int classes = (int)v.classes;
@@ -1260,9 +1258,10 @@ __global__ __launch_bounds__(256) void score_grad_col_kernel(LogitsView v, int64
 
 // Loss (a.loss) and / or gradient (grad) of a row; the gradient's scale: weight or the upstream gradient.  In float32, as a few classes
 // leave sums of a few roundings, but for what cancels: 1 - sum p, and the loss of a good student.  The exponentials relative to the row's maximum are kept for the gradient
-// (recomputed relative to the rest's maximum where the rest would underflow).
+// (recomputed relative to the rest's maximum where the rest would underflow).  Against 64 bits its losses and gradients are at 4e-7 of the
+// largest; the row family, whose few scalars are float64, at 6e-8.
 template <typename T, int CM, bool LOSS, bool GRAD>
-__global__ __launch_bounds__(256) void distill_col_kernel(LogitsView v, int64_t rows, DistillArgs a, T* __restrict__ grad) {
+__global__ __launch_bounds__(256, GRAD ? 1 : CM <= 24 ? 6 : CM <= 32 ? 5 : 1) void distill_col_kernel(LogitsView v, int64_t rows, DistillArgs a, T* __restrict__ grad) {
     const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (r >= rows) return;
     const int classes = (int)v.classes;
@@ -1301,7 +1300,7 @@ __global__ __launch_bounds__(256) void distill_col_kernel(LogitsView v, int64_t 
     const bool empty = m == -INFINITY;
     const double log_s = LOSS ? log((double)s) : (double)logf(s);
     u64 listed = 0;
-    bool bad = false;
+    bool bad = norm != norm || total != total;
     double sum = 0.0;
     for (int k = 0; k < a.k; ++k) {
         const int64_t i = load_int(a.index, l.base + k * l.stride, a.index_bytes);
@@ -1345,7 +1344,7 @@ __global__ __launch_bounds__(256) void distill_col_kernel(LogitsView v, int64_t 
         log_q_rest = shift + (LOSS ? log((double)s_rest) : (double)logf(s_rest)) - log_s;
         if (LOSS && rest > 0.f) sum += rest * (log((double)rest) - log_q_rest);
     }
-    const bool nan = bad || s != s || sum != sum || norm != norm || total != total;
+    const bool nan = bad || s != s || sum != sum;
     if (LOSS) a.loss[r] = w == 0.f ? 0.f : (nan ? NAN : (float)(sum * a.t * a.t)) * w;
     if (GRAD) {
         const float scale = (a.g_loss ? a.g_loss[r] : 1.f) * w * a.t;
@@ -1402,7 +1401,8 @@ template <bool READS, bool WRITES, typename F> static void by_once(const LogitsV
 
 bool score_is_col(const LogitsView& v) { return v.classes <= SCORE_COL_MAX; }
 
-// Fewer rows than compute units, of more than 16384 classes: cut so that about 256 blocks have work, no segment below 4096 classes.  With
+// Fewer rows than compute units, of more than 16384 classes: cut evenly so that about 256 blocks have work, into no more segments than there
+// are 4096 classes begun (16385 classes: four of 3328 and one of 3073).  With
 // twenty alternatives 4 x 128000 bf16 takes 11.8 us cut and 25.4 whole, 16 x 128000 12.4 and 25.6; 1 x 8000 10.7 and 7.8; without
 // alternatives 64 x 128000 8.8 and 14.1, 300 x 32000 as fast whole.  And no segment beyond what a block's bits take.
 SegPlan score_segments(const LogitsView& v, int64_t rows) {
@@ -1478,9 +1478,13 @@ void launch_score_grad(const LogitsView& v, int64_t rows, const void* tokens, in
     });
 }
 
-// Threads per row in distill_step_kernel; 0: rows are too few for a block each, or a block's bits do not cover them.  2048 / group rows
-// are in flight on each CU, and they have to fit the 256 MB of Infinity Cache: rows of 64 KB take 155 us at 256 threads (4096 of them)
-// and 204 at 1024, where the steps of a row are too short for so many waves; rows of 250 KB 534 at 512 and 509 at 1024.
+// Threads per row in distill_step_kernel; 0: rows are too few for a block each, or a block's bits do not cover them: then in two kernels.
+// 2048 / group rows are in flight on each CU, and they have to fit the 256 MB of Infinity Cache; in short rows the steps are too short for
+// many waves.  us of 4096 bf16 rows, lists of 64, at 256 / 512 / 1024 threads and in two kernels:
+//    32 KB   90   97  161   98       64 KB  154  158  219  176       96 KB  231  219  267  233      128 KB  298  283  317  297
+//   160 KB  394  344  362  354      192 KB  495  411  415  416      250 KB  638  537  524  548
+// and of rows that do not begin on 16 bytes: 65537 classes 346 322 381 360, 98305 classes 547 488 518 512.  The limits lie within 7 % of
+// the best of the four on both of their sides; 500 rows differ by less (250 KB: 82 81 83 86).
 static int step_group(const LogitsView& v, int64_t rows) {
     if (score_segments(v, rows).n > 1) return 0;
     if (wave_rows(v)) return 64;
