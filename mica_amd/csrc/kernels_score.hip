@@ -38,10 +38,10 @@ template <> __device__ __forceinline__ bf16_t from_f32<bf16_t>(float x) { return
 template <> __device__ __forceinline__ f16_t from_f32<f16_t>(float x) { return {(_Float16)x}; }
 
 // Which accesses bypass the caches (ONCE), by the size of the logits.  ONCE_STORE beyond 64 MB: what a gradient's stores would push out is
-// worth more to whoever runs next (gradient of 4096 x 32000 bf16 123 -> 104 us).  ONCE_BOTH, where the kernel does not read a row twice,
-// beyond 256 MB, the Infinity Cache, if all rows begin on 16 bytes: 4096 x 128000 bf16 200 -> 175 us, their gradient 402 -> 384; at 262 MB
-// nothing gained, and lost where a later pass would have found the rows cached, or where neighbouring lanes share the lines of unaligned
-// vectors (2048 x 50001 f16 66 -> 75 us).
+// worth more to whoever runs next (gradient of 4096 x 32000 bf16 117 -> 94 us, 1999 x 65537 f16 114 -> 92).  ONCE_BOTH, where the kernel does
+// not read a row twice, beyond 256 MB, the Infinity Cache, if all rows begin on 16 bytes: 4096 x 128000 bf16 scores 196 -> 176 us, loss 201 ->
+// 174, 8192 x 16384 f32 106 -> 92, a gradient the same (440); at 262 MB nothing gained, and lost where a later pass would have found the rows
+// cached, or where neighbouring lanes share the lines of unaligned vectors (2048 x 50001 f16 66 -> 75 us).
 enum { ONCE_NONE, ONCE_STORE, ONCE_BOTH };
 template <typename T> struct Vec { static constexpr int N = 16 / sizeof(T); };
 
@@ -709,7 +709,7 @@ __global__ __launch_bounds__(TOP ? JOIN : 64) void score_join_kernel(LogitsView 
 // ---- gradient of the scores ------------------------------------------------------------------------------------------------------------
 // dz_v = (1/T) [ g_lp ([v = t] - p_v) + g_lse p_v - g_H p_v (log p_v + H) ]: one read, one write.  p = 2^d / S with d = (z - m) c, from the
 // row's maximum m and sum S apart: a float32 log sum of a row of large magnitude has lost log S (a row of -1e9: all of it).  Streamed rows
-// get both from the forward pass, the column kernel has the classes in registers and sums again.  HBM-bound: 4096 x 32000 bf16 92 us = 5.7
+// get both from the forward pass, the column kernel has the classes in registers and sums again.  HBM-bound: 4096 x 32000 bf16 94 us = 5.6
 // TB/s, above the rate of a copy because the forward pass left part of the logits in the Infinity Cache.
 struct ScoreGrad {
     const void* tokens;
@@ -1019,7 +1019,7 @@ __device__ __forceinline__ RowGradient finish_row(const DistillArgs& a, ListLds 
 }
 
 // One read of the logits, a bit of LDS per class to leave out the listed ones (tail; subtracting them afterwards would cancel for every
-// good student).  HBM-bound: 4096 x 128000 bf16 174 us = 6.0 TB/s, 180 with the tail; 513 x 32003 15 us, the latency of its steps.
+// good student).  HBM-bound: 4096 x 128000 bf16 174 us = 6.0 TB/s, 185 with the tail and 64 entries; 513 x 32003 15 us, the latency of its steps.
 template <typename T, int G, bool TAIL, int ONCE>
 __global__ __launch_bounds__(256, (sizeof(T) == 4 ? 7 : 5) + (G == 256)) void distill_row_kernel(LogitsView v, int64_t rows, DistillArgs a, int segments, int seg_len, Partial* __restrict__ part) {
     constexpr int GROUPS = 256 / G;
@@ -1090,7 +1090,7 @@ struct Unlisted {
     __device__ __forceinline__ float operator()(float z) const { return none ? 0.f : f * exp2_hw(fmaf(z - sub, c, -R)); }
 };
 
-// One read, one write: 1999 x 65537 f16 92 us = 5.7 TB/s.
+// One read, one write: 1999 x 65537 f16 93 us = 5.6 TB/s.
 template <typename T, int G, int ONCE>
 __global__ __launch_bounds__(256) void distill_grad_row_kernel(LogitsView v, int64_t rows, DistillArgs a, int chunks, T* __restrict__ grad) {
     constexpr int GROUPS = 256 / G, CHUNK = G * UNROLL * Vec<T>::N;
@@ -1122,8 +1122,8 @@ __global__ __launch_bounds__(256) void distill_grad_row_kernel(LogitsView v, int
 }
 
 // Loss and gradient in one kernel: the row is read twice, the second time from cache, and its gradient written.  So that the second
-// read finds it there, G is chosen to leave few rows in flight: 2048 / G blocks on a CU (step_group).  4096 x 128000 bf16 489 us = 4.3 TB/s
-// of one read and one write; the two-kernel form takes 174 + 400, 256 threads per row 662 (the second read from HBM).  Holding the row in
+// read finds it there, G is chosen to leave few rows in flight: 2048 / G blocks on a CU (step_group).  4096 x 128000 bf16 495 us = 4.2 TB/s
+// of one read and one write; as a call 507, the two-kernel form 547, 256 threads per row 637 (the second read from HBM).  Holding the row in
 // the registers of 1024 threads took 562: one block on a CU, nothing to do while it sums.
 constexpr int STEP_U = 2;                                       // 64 registers: two blocks of 1024 threads on a CU
 template <typename T, int G, bool TAIL, int ONCE>
@@ -1185,9 +1185,9 @@ __global__ __launch_bounds__(G < 256 ? 256 : G, 8) void distill_step_kernel(Logi
 }
 
 // ========================================================================================================================================
-// rows of few classes, at any stride: a thread per row, the classes in registers.  8 x 20 x 64^3 f32 scores with three alternatives 54 us
-// = 4.8 TB/s, the gradient of 4 x 21 x 64^3 32 us = 5.5 TB/s; the distillation, whose list costs every class a comparison, is bound by its
-// instructions: loss 43 us, gradient 55 us for 4 x 21 x 64^3 with four entries.
+// rows of few classes, at any stride: a thread per row, the classes in registers.  8 x 20 x 64^3 f32 scores with three alternatives 55 us
+// = 4.8 TB/s, the gradient of 4 x 21 x 64^3 34 us = 5.2 TB/s; the distillation, whose list costs every class a comparison, is bound by its
+// instructions: loss 45 us, gradient 56 us for 4 x 21 x 64^3 with four entries.
 // ========================================================================================================================================
 template <int CM, typename T> __device__ __forceinline__ void load_classes(float (&z)[CM], const T* p, int64_t sc, int classes) {
 #pragma unroll
@@ -1258,8 +1258,8 @@ __global__ __launch_bounds__(256, 6) void score_grad_col_kernel(LogitsView v, in
 
 // Loss (a.loss) and / or gradient (grad) of a row; the gradient's scale: weight or the upstream gradient.  In float32, as a few classes
 // leave sums of a few roundings, but for what cancels: 1 - sum p, and the loss of a good student.  The exponentials relative to the row's maximum are kept for the gradient
-// (recomputed relative to the rest's maximum where the rest would underflow).  Against 64 bits its losses and gradients are at 4e-7 of the
-// largest; the row family, whose few scalars are float64, at 6e-8.
+// (recomputed relative to the rest's maximum where the rest would underflow).  Against 64 bits its losses and gradients are
+// off by 4e-7 to 9e-7 (relative, over a tensor); the row family's, whose few scalars are float64, by 6e-8.
 template <typename T, int CM, bool LOSS, bool GRAD>
 __global__ __launch_bounds__(256, GRAD ? 1 : CM <= 24 ? 6 : CM <= 32 ? 5 : 1) void distill_col_kernel(LogitsView v, int64_t rows, DistillArgs a, T* __restrict__ grad) {
     const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -1481,10 +1481,10 @@ void launch_score_grad(const LogitsView& v, int64_t rows, const void* tokens, in
 // Threads per row in distill_step_kernel; 0: rows are too few for a block each, or a block's bits do not cover them: then in two kernels.
 // 2048 / group rows are in flight on each CU, and they have to fit the 256 MB of Infinity Cache; in short rows the steps are too short for
 // many waves.  us of 4096 bf16 rows, lists of 64, at 256 / 512 / 1024 threads and in two kernels:
-//    32 KB   90   97  161   98       64 KB  154  158  219  176       96 KB  231  219  267  233      128 KB  298  283  317  297
-//   160 KB  394  344  362  354      192 KB  495  411  415  416      250 KB  638  537  524  548
-// and of rows that do not begin on 16 bytes: 65537 classes 346 322 381 360, 98305 classes 547 488 518 512.  The limits lie within 7 % of
-// the best of the four on both of their sides; 500 rows differ by less (250 KB: 82 81 83 86).
+//    32 KB   88   95  151   98       64 KB  150  152  205  175       96 KB  228  214  252  231      128 KB  297  277  301  299
+//   160 KB  394  337  346  355      192 KB  492  400  402  421      250 KB  637  527  507  547
+// and of rows that do not begin on 16 bytes: 65537 classes 342 317 360 360, 98305 classes 545 481 508 509.  The limits lie within 8 % of
+// the best of the four on both of their sides; 500 rows differ by less (250 KB: 81 79 81 86).
 static int step_group(const LogitsView& v, int64_t rows) {
     if (score_segments(v, rows).n > 1) return 0;
     if (wave_rows(v)) return 64;
